@@ -94,6 +94,19 @@ _SIGS = {
                                     c_int, c_void_p]),
     "dlm_bitlinear": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
                               c_void_p, c_void_p]),
+    "dlm_add_rms_norm_i8": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                    c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_void_p]),
+    "dlm_gemm_i8": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                            c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "dlm_kv_i8_append": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                 c_int, c_void_p]),
+    "dlm_kv_i8_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                               c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
+                               c_void_p]),
+    "dlm_attention_kv_i8": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                    c_void_p, c_void_p, c_int, c_float, c_int, c_void_p]),
     "dlm_unet_create": (c_int, [ctypes.POINTER(c_int), c_int, c_int, ctypes.POINTER(c_char_p),
                                 ctypes.POINTER(c_void_p), ctypes.POINTER(ctypes.c_int64),
                                 ctypes.POINTER(c_void_p), c_void_p]),
@@ -148,6 +161,11 @@ _SIGS = {
     "dlm_vae_weight_info": (c_int, [c_int, ctypes.c_char_p, c_int, ctypes.POINTER(ctypes.c_int64),
                                     ctypes.POINTER(c_int)]),
 }
+
+# dlm_dtype
+F32 = 0
+F16 = 1
+BF16 = 2
 
 EPI_BIAS = 1
 EPI_RESID = 2

@@ -24,6 +24,7 @@ enum DeviceStatus : int {
   kDevTimeoutEpilogue = 3,
   kDevTimeoutSoftmax = 4,
   kDevTimeoutStreamK = 5,  // a stream-K tile owner gave up waiting for a partial accumulator
+  kDevBadPosition = 6,     // an int8 cache call was given a position or length outside the cache
 };
 
 }  // namespace dlm

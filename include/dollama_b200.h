@@ -39,6 +39,13 @@ typedef enum dlm_status {
 
 /* ------------------------------------------------------------------ library */
 
+/* Element types of the operators that take a `dtype` (others name theirs). */
+typedef enum dlm_dtype {
+  DLM_F32 = 0,
+  DLM_F16 = 1,  /* IEEE binary16 */
+  DLM_BF16 = 2  /* bfloat16      */
+} dlm_dtype;
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* dlm_last_error(void);
 
@@ -46,7 +53,8 @@ const char* dlm_last_error(void);
 const char* dlm_version(void);
 
 /* Reads (and clears when `clear` != 0) the device status word of the current device:
- * 0 = no kernel gave up a wait; otherwise the code of the first kernel role that timed out.
+ * 0 = no kernel gave up a wait; 1..5 = the code of the first kernel role that timed out; 6 = an
+ * int8 cache call was given a position or a length outside its cache (those rows were skipped).
  * Synchronizes `stream`. */
 int dlm_get_device_status(int* out_code, int clear, void* stream);
 
@@ -315,6 +323,73 @@ int dlm_bitnet_generate(void* handle, const int* prompts, int B, int P, int max_
 int dlm_bitnet_weight_count(const dlm_bitnet_config* cfg);
 int dlm_bitnet_weight_info(const dlm_bitnet_config* cfg, int index, char* name, int name_cap,
                            int64_t* shape, int* ndim);
+
+/* ---------------------------------------------------- int8 operators of a language-model layer
+ *
+ * A decoder layer with int8 activations (one scale per token), int8 weights (one scale per output
+ * channel) and an int8 K/V cache (one scale per token and head), for any model dimensions:
+ *   dlm_add_rms_norm_i8 -> dlm_gemm_i8 (q|k|v) -> dlm_kv_i8_append -> dlm_attention_kv_i8 ->
+ *   dlm_quantize_act_i8 -> dlm_gemm_i8 (out) -> dlm_add_rms_norm_i8 -> ...
+ * The reference has no counterpart (its LM is ternary with an fp32 cache).  `dtype` is a dlm_dtype.
+ * Row strides (ld*) are in elements.  int8 codes follow dlm_quantize_act_i8: with a = max|x| over
+ * the row, scale = a / 127 and code = round(127 x / a), halves away from zero; an all-zero row has
+ * scale 0 and codes 0; a row with a NaN or an infinity has scale NaN and codes 0, so that whatever
+ * is computed from it is NaN.  Weights are quantized per channel by dlm_quantize_act_i8 on [N, K].
+ * No call allocates, synchronises or keeps state: all may be captured into CUDA graphs, and calls
+ * on different streams may overlap as long as their outputs are distinct.
+ */
+
+/* RMS norm with the residual's addition, and an int8 output:
+ *   h[m, k] = T(x[m, k] + residual[m, k])  (residual may be NULL: h = x; h_out may be NULL: not
+ *             stored; h_out may be x or residual, with the same stride)
+ *   xq, xscale = codes and scale of the row h[m, :] * weight[:] / sqrt(mean_k h[m, k]^2 + eps)
+ * x, residual, weight and h_out are of `dtype`; xq is [M, K] contiguous, xscale [M].  h is rounded
+ * to `dtype` before it is normed.  Codes are exact: those of the formula without roundings
+ * (fp32 inputs: with the products in double).  K <= 32768, eps > 0, any alignment of the elements;
+ * rows that all start on 16-byte boundaries are faster. */
+int dlm_add_rms_norm_i8(const void* x, int ldx, const void* residual, int ldr, const void* weight,
+                        void* h_out, int ldh, int8_t* xq, float* xscale, int M, int K, float eps,
+                        int dtype, void* stream);
+
+/* Matrix product in 8-bit integers with a scale for each token and each channel:
+ *   y[m, n] = T(float(sum_k xq[m, k] w[n, k]) * xscale[m] * wscale[n] + bias[n])
+ * xq [M, K] (row stride ldx), w [N, K] contiguous, xscale [M], wscale [N], bias [N] of `dtype` or
+ * NULL, y [M, N] of `dtype` (row stride ldy; the elements between rows stay).  The integer sum is
+ * exact, the epilogue fp32.  K and ldx multiples of 16, K < 131072, xq and w 16-byte aligned;
+ * any M and N. */
+int dlm_gemm_i8(const int8_t* xq, int ldx, const float* xscale, const int8_t* w, const float* wscale,
+                const void* bias, void* y, int ldy, int M, int N, int K, int dtype, void* stream);
+
+/* int8 K/V cache: codes kq, vq [B, H, Lmax, Dh], scales kscale, vscale [B, H, Lmax].
+ * append quantizes the rows k, v of new tokens ([B * S] tokens of stride ldk / ldv, head h in
+ * columns [h * Dh, (h + 1) * Dh): columns of a q|k|v projection may be passed as they are) into
+ * positions pos[b] + s of sequence b, for s < counts[b] (counts NULL: all S tokens); read writes
+ * the same rows' values, T(code * scale), back to k, v.  Everything else stays as it was: tokens
+ * from counts[b] on, other cache rows.  A token whose position falls outside [0, Lmax) is skipped
+ * and raises the device status word (code 6).  pos, counts: device int32 [B].  Dh 64 or 128; k and
+ * v rows on 16-byte boundaries; each (sequence, position) at most once per call. */
+int dlm_kv_i8_append(const void* k, int ldk, const void* v, int ldv, int8_t* kq, float* kscale,
+                     int8_t* vq, float* vscale, int B, int S, int H, int Dh, int Lmax, const int* pos,
+                     const int* counts, int dtype, void* stream);
+int dlm_kv_i8_read(const int8_t* kq, const float* kscale, const int8_t* vq, const float* vscale,
+                   void* k, int ldk, void* v, int ldv, int B, int S, int H, int Dh, int Lmax,
+                   const int* pos, const int* counts, int dtype, void* stream);
+
+/* Attention of new tokens over that cache (which holds their own keys already):
+ *   out = softmax(scale q k^T) v,  k and v the values the cache stands for,
+ * q, out [B * Sq] tokens of stride ldq / ldo with head h in columns [h * Dh, (h + 1) * Dh), head h
+ * reading kv head h / (Hq / Hkv).  Sequence b has kv_len[b] cached tokens and q_len[b] <= Sq queries
+ * (q_len NULL: Sq), which with causal != 0 are its last tokens: query i sees keys
+ * [0, kv_len[b] - q_len[b] + i]; with causal == 0 every query sees keys [0, kv_len[b]).  A query
+ * that sees no key gets zeros; queries from q_len[b] on are not written; keys that a query does not
+ * see do not touch its result, whatever they hold.  A kv_len outside [0, Lmax] is clamped and
+ * raises the device status word (code 6).  kv_len, q_len: device int32 [B].  Dh 64 or 128; q and out
+ * rows on 16-byte boundaries.  Softmax statistics and sums are fp32; fp32 inputs keep 22 bits or
+ * more of q and of the weights, 16-bit inputs 11 of the weights. */
+int dlm_attention_kv_i8(const void* q, int ldq, const int8_t* kq, const float* kscale,
+                        const int8_t* vq, const float* vscale, void* out, int ldo, int B, int Hq,
+                        int Hkv, int Sq, int Dh, int Lmax, const int* kv_len, const int* q_len,
+                        int causal, float scale, int dtype, void* stream);
 
 /* ------------------------------------------------------------------ SDXL UNet (model level)
  *
