@@ -40,15 +40,36 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
-// The absmax int8 code of x in a row of largest magnitude a, round_half_away(127 x / a), given
-// v = x * (127 / a) in fp32.  v is within 2^-15 of the quotient (three roundings of at most
-// 127 * 2^-24 each), so away from a half-integer it rounds as the quotient does; next to one the
-// quotient is formed in double, where 127 * x is exact for products of up to 46 bits and the
-// correctly rounded division returns an exact tie as one.
-__device__ __forceinline__ int quant_code(float v, double x, double a) {
-  const int q = __float2int_rn(v);
-  const float d = fabsf(v - static_cast<float>(q));
-  if (d < 0.5f - 0x1p-13f) return q;
+// The absmax int8 codes round_half_away(127 x_j / a) of N values (a multiple of 4) of a row of
+// largest magnitude a, given v_j = x_j * (127 / a) in fp32, which is within `err` of the quotient:
+// away from a half-integer v_j rounds as the quotient does.  Next to one `exact(j)` forms the
+// quotient in double (quant_exact), on a branch that few vectors take (two in 10^3 for eight values
+// and err 2^-14).  Rounding is the addition of 3 * 2^22, whose sum's low byte is the code.
+template <int N, typename F>
+__device__ __forceinline__ void quant_codes(const float (&v)[N], float err, uint32_t (&out)[N / 4], F&& exact) {
+  constexpr float kMagic = 12582912.0f;
+  uint32_t t[N];
+  float far = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float r = __fadd_rn(v[j], kMagic);
+    t[j] = __float_as_uint(r);
+    far = fmaxf(far, fabsf(__fsub_rn(v[j], __fsub_rn(r, kMagic))));
+  }
+  if (far >= 0.5f - err) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (fabsf(__fsub_rn(v[j], __fsub_rn(__uint_as_float(t[j]), kMagic))) >= 0.5f - err)
+        t[j] = static_cast<uint32_t>(exact(j));
+  }
+#pragma unroll
+  for (int j = 0; j < N; j += 4)
+    out[j / 4] = __byte_perm(__byte_perm(t[j], t[j + 1], 0x0040), __byte_perm(t[j + 2], t[j + 3], 0x0040), 0x5410);
+}
+
+// The same code from double: 127 x is exact for x of up to 46 bits, and the correctly rounded
+// division returns an exact tie as one.
+__device__ __forceinline__ int quant_exact(double x, double a) {
   return static_cast<int>(round(__ddiv_rn(__dmul_rn(127.0, x), a)));
 }
 

@@ -4,12 +4,12 @@
 // One row is the Dh values of one token and one head; its scale is a / 127 (a = largest magnitude)
 // and its codes round_half_away(127 x / a), the rule of dlm_quantize_act_i8.  Codes are
 // [B][H][Lmax][Dh], scales [B][H][Lmax], so a head's keys are contiguous for the attention that
-// reads them.  A row is handled by Dh / 8 neighbouring lanes, 8 values each: reads of 16 or 32 bytes
-// a lane, one shuffle tree for the largest magnitude, 8-byte code stores.  Memory-bound.
+// reads them.  Dh / 8 neighbouring lanes take the K row and the V row of one token and head, 8
+// values each: 16 or 32 bytes a lane and row, one shuffle tree for the two largest magnitudes, 8-byte
+// code stores.  Memory-bound.
 #include <cstdint>
 
 #include "dtype.cuh"
-#include "kv_i8.h"
 #include "ptx.cuh"
 
 namespace dlm {
@@ -18,18 +18,51 @@ namespace {
 
 constexpr int kKvThreads = 256;
 
-template <typename T>
-struct Oct {  // 8 elements in 16-byte pieces
-  static constexpr int kPieces = sizeof(T) / 2;
-  Vec<T, 16 / sizeof(T)> v[kPieces];
-  __device__ __forceinline__ T& at(int i) { return v[i / (16 / sizeof(T))].v[i % (16 / sizeof(T))]; }
+// n / d for n < 2^31 by a multiplication: q = (umulhi(n, mul) + n) >> shift with shift =
+// ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
+struct FastDiv {
+  unsigned d, mul, shift;
+  explicit FastDiv(unsigned v) : d(v), mul(0), shift(0) {
+    while ((1ull << shift) < v) ++shift;
+    mul = static_cast<unsigned>(((1ull << 32) * ((1ull << shift) - v)) / v + 1);
+  }
+  __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
 };
 
-// The cache row of (token b, s; head) and whether it exists: s below the sequence's count and its
-// position inside the cache (a position outside raises the device status word).
-__device__ __forceinline__ bool cache_row(const KvShape& p, int b, int s, int hd, size_t& row) {
-  const int n = p.counts ? p.counts[b] : p.S;
-  if (s >= n) return false;
+struct KvShape {
+  int B, S, H, Lmax;
+  const int* pos;     // [B] position of each sequence's first new token
+  const int* counts;  // [B] new tokens of each sequence, or null: S
+  int* status;        // device status word
+  unsigned units;     // B * S * H
+  FastDiv by_h, by_s;
+};
+
+// 8 elements of a row in 16-byte pieces
+template <typename T>
+struct Oct {
+  static constexpr int kPer = 16 / sizeof(T), kPieces = 8 / kPer;
+  Vec<T, kPer> v[kPieces];
+  __device__ __forceinline__ T& at(int i) { return v[i / kPer].v[i % kPer]; }
+  __device__ __forceinline__ void load(const T* src) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) v[j] = reinterpret_cast<const Vec<T, kPer>*>(src)[j];
+  }
+  __device__ __forceinline__ void store(T* dst) const {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) reinterpret_cast<Vec<T, kPer>*>(dst)[j] = v[j];
+  }
+};
+
+// Unit u is (token, head).  Whether its cache row exists: the token is below its sequence's count and
+// its position inside the cache (a position outside raises the device status word).
+__device__ __forceinline__ bool locate(const KvShape& p, unsigned u, unsigned& tok, unsigned& hd, size_t& row) {
+  if (u >= p.units) return false;
+  tok = p.by_h.div(u);
+  hd = u - tok * p.H;
+  const unsigned b = p.by_s.div(tok);
+  const int s = static_cast<int>(tok - b * p.S);
+  if (s >= (p.counts ? p.counts[b] : p.S)) return false;
   const long long at = static_cast<long long>(p.pos[b]) + s;
   if (at < 0 || at >= p.Lmax) {
     if (p.status) atomicCAS(p.status, 0, kDevBadPosition);
@@ -39,6 +72,29 @@ __device__ __forceinline__ bool cache_row(const KvShape& p, int b, int s, int hd
   return true;
 }
 
+// Codes of this lane's 8 values and their store; a: the row's largest magnitude (or NaN).
+template <typename T>
+__device__ __forceinline__ void write_row(Oct<T>& x, float a, int8_t* q, float* scale, bool first) {
+  const bool finite = a < INFINITY;  // false for a NaN as well
+  const double da = static_cast<double>(a);
+  auto exact = [&](int j) { return quant_exact(static_cast<double>(to_f(x.at(j))), da); };
+  uint32_t c[2] = {0, 0};
+  if (a >= 1e-30f && finite) {
+    const float rq = 127.0f / a;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f(x.at(j)) * rq;
+    quant_codes<8>(v, 0x1p-15f, c, exact);  // two roundings: within 127 * 2^-23
+  } else if (a > 0.0f && finite) {
+    // 127 / a may leave fp32's range
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j / 4] |= (static_cast<uint32_t>(exact(j)) & 0xFFu) << (8 * (j % 4));
+  }
+  *reinterpret_cast<uint2*>(q) = make_uint2(c[0], c[1]);
+  // a row that holds a NaN or an infinity: codes 0 under a NaN scale
+  if (first) *scale = finite ? __fdiv_rn(a, 127.0f) : NAN;
+}
+
 template <typename T, int DH>
 __global__ void __launch_bounds__(kKvThreads)
     kv_append_kernel(const T* __restrict__ k, long long ldk, const T* __restrict__ v, long long ldv,
@@ -46,50 +102,41 @@ __global__ void __launch_bounds__(kKvThreads)
                      float* __restrict__ vs, const KvShape p) {
   griddep_wait();  // inputs come from the previous kernel (programmatic dependent launch)
   constexpr int G = DH / 8;
-  const long long u = (static_cast<long long>(blockIdx.x) * kKvThreads + threadIdx.x) / G;
+  const unsigned u = blockIdx.x * (kKvThreads / G) + threadIdx.x / G;
   const int c = threadIdx.x % G;
-  const long long rows = static_cast<long long>(p.B) * p.S * p.H;
-  // unit u: K row u, then (from `rows` on) V row u - rows
-  const bool is_v = u >= rows;
-  const long long i = is_v ? u - rows : u;
+  unsigned tok = 0, hd = 0;
   size_t row = 0;
-  bool live = u < 2 * rows;
-  int hd = 0;
-  long long tok = 0;
+  const bool live = locate(p, u, tok, hd, row);
+  Oct<T> xk, xv;
+  float ak = 0.0f, av = 0.0f;
   if (live) {
-    hd = static_cast<int>(i % p.H);
-    tok = i / p.H;
-    live = cache_row(p, static_cast<int>(tok / p.S), static_cast<int>(tok % p.S), hd, row);
-  }
-  Oct<T> x;
-  float a = 0.0f;
-  if (live) {
-    const T* src = (is_v ? v + tok * ldv : k + tok * ldk) + hd * DH + c * 8;
+    xk.load(k + tok * ldk + hd * DH + c * 8);
+    xv.load(v + tok * ldv + hd * DH + c * 8);
 #pragma unroll
-    for (int j = 0; j < Oct<T>::kPieces; ++j)
-      x.v[j] = reinterpret_cast<const Vec<T, 16 / sizeof(T)>*>(src)[j];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a = max_nan(a, fabsf(to_f(x.at(j))));
+    for (int j = 0; j < 8; ++j) {
+      ak = max_nan(ak, fabsf(to_f(xk.at(j))));
+      av = max_nan(av, fabsf(to_f(xv.at(j))));
+    }
   }
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+  for (int o = G / 2; o > 0; o >>= 1) {
+    ak = max_nan(ak, __shfl_xor_sync(0xffffffffu, ak, o));
+    av = max_nan(av, __shfl_xor_sync(0xffffffffu, av, o));
+  }
   if (!live) return;
-  const bool finite = a < INFINITY;  // false for a NaN as well
-  const bool tiny = a < 1e-30f;      // 127 / a may leave fp32's range: quotients in double
-  const float rq = 127.0f / a;
-  Vec<int8_t, 8> q;
+  write_row(xk, ak, kq + row * DH + c * 8, ks + row, c == 0);
+  write_row(xv, av, vq + row * DH + c * 8, vs + row, c == 0);
+}
+
+template <typename T>
+__device__ __forceinline__ Oct<T> values(uint2 q, float scale) {
+  Oct<T> x;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float f = to_f(x.at(j));
-    int code = 0;
-    if (finite && a > 0.0f)
-      code = tiny ? static_cast<int>(round(__ddiv_rn(127.0 * static_cast<double>(f), static_cast<double>(a))))
-                  : quant_code(f * rq, static_cast<double>(f), static_cast<double>(a));
-    q.v[j] = static_cast<int8_t>(code);
+    const int code = static_cast<int>((j < 4 ? q.x : q.y) << (24 - 8 * (j % 4))) >> 24;
+    x.at(j) = from_f<T>(static_cast<float>(code) * scale);
   }
-  *reinterpret_cast<Vec<int8_t, 8>*>((is_v ? vq : kq) + row * DH + c * 8) = q;
-  // a row that holds a NaN or an infinity: codes 0 under a NaN scale
-  if (c == 0) (is_v ? vs : ks)[row] = finite ? __fdiv_rn(a, 127.0f) : NAN;
+  return x;
 }
 
 template <typename T, int DH>
@@ -99,48 +146,48 @@ __global__ void __launch_bounds__(kKvThreads)
                    long long ldk, T* __restrict__ v, long long ldv, const KvShape p) {
   griddep_wait();  // inputs come from the previous kernel (programmatic dependent launch)
   constexpr int G = DH / 8;
-  const long long u = (static_cast<long long>(blockIdx.x) * kKvThreads + threadIdx.x) / G;
+  const unsigned u = blockIdx.x * (kKvThreads / G) + threadIdx.x / G;
   const int c = threadIdx.x % G;
-  const long long rows = static_cast<long long>(p.B) * p.S * p.H;
-  if (u >= 2 * rows) return;
-  const bool is_v = u >= rows;
-  const long long i = is_v ? u - rows : u;
-  const int hd = static_cast<int>(i % p.H);
-  const long long tok = i / p.H;
+  unsigned tok, hd;
   size_t row;
-  if (!cache_row(p, static_cast<int>(tok / p.S), static_cast<int>(tok % p.S), hd, row)) return;
-  const float sc = (is_v ? vs : ks)[row];
-  const Vec<int8_t, 8> q = *reinterpret_cast<const Vec<int8_t, 8>*>((is_v ? vq : kq) + row * DH + c * 8);
-  Oct<T> x;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x.at(j) = from_f<T>(static_cast<float>(q.v[j]) * sc);
-  T* dst = (is_v ? v + tok * ldv : k + tok * ldk) + hd * DH + c * 8;
-#pragma unroll
-  for (int j = 0; j < Oct<T>::kPieces; ++j) reinterpret_cast<Vec<T, 16 / sizeof(T)>*>(dst)[j] = x.v[j];
+  if (!locate(p, u, tok, hd, row)) return;
+  const uint2 qk = *reinterpret_cast<const uint2*>(kq + row * DH + c * 8);
+  const uint2 qv = *reinterpret_cast<const uint2*>(vq + row * DH + c * 8);
+  const float sk = ks[row], sv = vs[row];
+  values<T>(qk, sk).store(k + tok * ldk + hd * DH + c * 8);
+  values<T>(qv, sv).store(v + tok * ldv + hd * DH + c * 8);
 }
 
+// The host checks of both calls; `empty` when there is nothing to do.
 int check(const char* fn, const void* k, int ldk, const void* v, int ldv, const void* kq, const void* ks,
-          const void* vq, const void* vs, const KvShape& p, int Dh, int dtype) {
-  DLM_REQUIRE(p.B >= 0 && p.S >= 0 && p.H >= 0 && p.Lmax >= 0, DLM_ERR_INVALID, "%s: negative size", fn);
+          const void* vq, const void* vs, int B, int S, int H, int Dh, int Lmax, const int* pos, int dtype,
+          bool& empty) {
+  empty = false;
+  DLM_REQUIRE(B >= 0 && S >= 0 && H >= 0 && Lmax >= 0, DLM_ERR_INVALID, "%s: negative size", fn);
   DLM_REQUIRE(dtype_ok(dtype), DLM_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
   DLM_REQUIRE(Dh == 64 || Dh == 128, DLM_ERR_UNSUPPORTED, "%s: head dim %d (64 or 128)", fn, Dh);
-  if (p.B == 0 || p.S == 0 || p.H == 0 || p.Lmax == 0) return DLM_OK;
-  DLM_REQUIRE(k && v && kq && ks && vq && vs && p.pos, DLM_ERR_INVALID, "%s: null pointer", fn);
-  const long long width = static_cast<long long>(p.H) * Dh;
+  empty = B == 0 || S == 0 || H == 0 || Lmax == 0;
+  if (empty) return DLM_OK;
+  DLM_REQUIRE(k && v && kq && ks && vq && vs && pos, DLM_ERR_INVALID, "%s: null pointer", fn);
+  const long long width = static_cast<long long>(H) * Dh;
   DLM_REQUIRE(ldk >= width && ldv >= width, DLM_ERR_INVALID, "%s: a token stride is below H * Dh = %lld", fn,
               width);
   const int vec = static_cast<int>(16 / dtype_size(dtype));
   DLM_REQUIRE(aligned16(k) && aligned16(v) && ldk % vec == 0 && ldv % vec == 0, DLM_ERR_INVALID,
               "%s: k / v rows must start on 16-byte boundaries", fn);
   DLM_REQUIRE(aligned16(kq) && aligned16(vq), DLM_ERR_INVALID, "%s: cache codes must be 16-byte aligned", fn);
-  DLM_REQUIRE(2ll * p.B * p.S * p.H * (Dh / 8) / kKvThreads < (1ll << 31) - 1, DLM_ERR_UNSUPPORTED,
-              "%s: too many rows", fn);
+  DLM_REQUIRE(static_cast<double>(B) * S * H < 2147483000.0, DLM_ERR_UNSUPPORTED, "%s: too many rows", fn);
   return DLM_OK;
 }
 
-unsigned grid_of(const KvShape& p, int Dh) {
-  const long long threads = 2ll * p.B * p.S * p.H * (Dh / 8);
-  return static_cast<unsigned>((threads + kKvThreads - 1) / kKvThreads);
+KvShape shape(int B, int S, int H, int Lmax, const int* pos, const int* counts) {
+  return KvShape{B, S, H, Lmax, pos, counts, device_status_ptr(), static_cast<unsigned>(B) * S * H,
+                 FastDiv(H), FastDiv(S)};
+}
+
+dim3 grid_of(const KvShape& p, int Dh) {
+  const unsigned per = kKvThreads / (Dh / 8);
+  return dim3((p.units + per - 1) / per);
 }
 
 }  // namespace
@@ -153,21 +200,15 @@ int dlm_kv_i8_append(const void* k, int ldk, const void* v, int ldv, int8_t* kq,
                      float* vscale, int B, int S, int H, int Dh, int Lmax, const int* pos,
                      const int* counts, int dtype, void* stream) {
   using namespace dlm;
-  KvShape p{B, S, H, Lmax, pos, counts, nullptr};
-  const int rc = check("kv_i8_append", k, ldk, v, ldv, kq, kscale, vq, vscale, p, Dh, dtype);
-  if (rc != DLM_OK || B == 0 || S == 0 || H == 0 || Lmax == 0) return rc;
-  p.status = device_status_ptr();
-  const dim3 grid(grid_of(p, Dh));
+  bool empty;
+  const int rc = check("kv_i8_append", k, ldk, v, ldv, kq, kscale, vq, vscale, B, S, H, Dh, Lmax, pos, dtype, empty);
+  if (rc != DLM_OK || empty) return rc;
+  const KvShape p = shape(B, S, H, Lmax, pos, counts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DLM_DISPATCH_DTYPE(dtype, T, {
-    const T* kt = static_cast<const T*>(k);
-    const T* vt = static_cast<const T*>(v);
-    if (Dh == 64)
-      DLM_CHECK_CUDA(launch_pdl(kv_append_kernel<T, 64>, grid, dim3(kKvThreads), 0, s, kt, ldk, vt, ldv, kq,
-                                kscale, vq, vscale, p));
-    else
-      DLM_CHECK_CUDA(launch_pdl(kv_append_kernel<T, 128>, grid, dim3(kKvThreads), 0, s, kt, ldk, vt, ldv, kq,
-                                kscale, vq, vscale, p));
+    auto kernel = Dh == 64 ? kv_append_kernel<T, 64> : kv_append_kernel<T, 128>;
+    DLM_CHECK_CUDA(launch_pdl(kernel, grid_of(p, Dh), dim3(kKvThreads), 0, s, static_cast<const T*>(k), ldk,
+                              static_cast<const T*>(v), ldv, kq, kscale, vq, vscale, p));
   });
   return DLM_OK;
 }
@@ -176,21 +217,15 @@ int dlm_kv_i8_read(const int8_t* kq, const float* kscale, const int8_t* vq, cons
                    int ldk, void* v, int ldv, int B, int S, int H, int Dh, int Lmax, const int* pos,
                    const int* counts, int dtype, void* stream) {
   using namespace dlm;
-  KvShape p{B, S, H, Lmax, pos, counts, nullptr};
-  const int rc = check("kv_i8_read", k, ldk, v, ldv, kq, kscale, vq, vscale, p, Dh, dtype);
-  if (rc != DLM_OK || B == 0 || S == 0 || H == 0 || Lmax == 0) return rc;
-  p.status = device_status_ptr();
-  const dim3 grid(grid_of(p, Dh));
+  bool empty;
+  const int rc = check("kv_i8_read", k, ldk, v, ldv, kq, kscale, vq, vscale, B, S, H, Dh, Lmax, pos, dtype, empty);
+  if (rc != DLM_OK || empty) return rc;
+  const KvShape p = shape(B, S, H, Lmax, pos, counts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DLM_DISPATCH_DTYPE(dtype, T, {
-    T* kt = static_cast<T*>(k);
-    T* vt = static_cast<T*>(v);
-    if (Dh == 64)
-      DLM_CHECK_CUDA(launch_pdl(kv_read_kernel<T, 64>, grid, dim3(kKvThreads), 0, s, kq, kscale, vq, vscale,
-                                kt, ldk, vt, ldv, p));
-    else
-      DLM_CHECK_CUDA(launch_pdl(kv_read_kernel<T, 128>, grid, dim3(kKvThreads), 0, s, kq, kscale, vq, vscale,
-                                kt, ldk, vt, ldv, p));
+    auto kernel = Dh == 64 ? kv_read_kernel<T, 64> : kv_read_kernel<T, 128>;
+    DLM_CHECK_CUDA(launch_pdl(kernel, grid_of(p, Dh), dim3(kKvThreads), 0, s, kq, kscale, vq, vscale,
+                              static_cast<T*>(k), ldk, static_cast<T*>(v), ldv, p));
   });
   return DLM_OK;
 }

@@ -42,7 +42,7 @@ __device__ __forceinline__ double max_nan_d(double a, double b) { return (a > b 
 // + VEC - 1 of step i.  NV > 0: at most NV steps, h in registers; NV == 0: any number, h in dynamic
 // shared memory (each thread reads only what it wrote).
 template <int NV>
-constexpr int kNormMaxThreads = NV == 1 || NV == 2 ? 256 : NV == 4 ? 512 : 1024;
+constexpr int kNormMaxThreads = NV == 1 || NV == 2 ? 256 : 512;
 
 template <typename T, int VEC, int NV>
 __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(const NormParams p) {
@@ -52,7 +52,6 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
   __shared__ double s_dsum[32], s_dmax[32];
   const int nw = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   using V = Vec<T, VEC>;
-  using Q = Vec<int8_t, VEC>;
   const T* w = static_cast<const T*>(p.w);
   const int row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx;
@@ -175,19 +174,33 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
     const int k = (i * blockDim.x + threadIdx.x) * VEC;
     if (k >= p.K) continue;
     const V wv = *reinterpret_cast<const V*>(w + k);
-    Q c;
+    const V hv = H(i);
+    auto exact = [&](int j) {
+      return quant_exact(static_cast<double>(to_f(hv.v[j])) * static_cast<double>(to_f(wv.v[j])), damax);
+    };
+    // 127 / a and its product: within 127 * 2^-23 for exact products and a, twice that otherwise
+    constexpr float kErr = kWide ? 0x1p-14f : 0x1p-15f;
+    constexpr int N = VEC < 4 ? 4 : VEC;
+    float v[N];
+    uint32_t c[N / 4];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float f = to_f(H(i).v[j]), wf = to_f(wv.v[j]);
-      const double d = static_cast<double>(f) * static_cast<double>(wf);
-      if (plain)
-        c.v[j] = static_cast<int8_t>(quant_code(f * wf * rq, d, damax));
-      else
-        c.v[j] = damax > 0.0 && dscale == dscale
-                     ? static_cast<int8_t>(static_cast<int>(round(__ddiv_rn(__dmul_rn(127.0, d), damax))))
-                     : static_cast<int8_t>(0);
+    for (int j = 0; j < N; ++j) v[j] = j < VEC ? to_f(hv.v[j < VEC ? j : 0]) * to_f(wv.v[j < VEC ? j : 0]) * rq : 0.0f;
+    if (plain) {
+      quant_codes<N>(v, kErr, c, exact);
+    } else {
+      const bool some = damax > 0.0 && dscale == dscale;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint32_t code = j < VEC && some ? static_cast<uint32_t>(exact(j < VEC ? j : 0)) & 0xFFu : 0u;
+        c[j / 4] = (j % 4 ? c[j / 4] : 0u) | code << (8 * (j % 4));
+      }
     }
-    *reinterpret_cast<Q*>(qo + k) = c;
+    if constexpr (VEC < 4)
+      qo[k] = static_cast<int8_t>(c[0] & 0xFFu);
+    else if constexpr (VEC == 4)
+      *reinterpret_cast<uint32_t*>(qo + k) = c[0];
+    else
+      *reinterpret_cast<uint2*>(qo + k) = make_uint2(c[0], c[1]);
   }
 }
 
@@ -198,22 +211,20 @@ int launch_norm(const NormParams& p, cudaStream_t s) {
     const int threads = ((n + nv - 1) / nv + 31) / 32 * 32;
     return launch_pdl(kernel, dim3(p.M), dim3(threads), 0, s, p);
   };
-  if constexpr (VEC == 1) {
-    const int threads = n >= 4096 ? 1024 : n >= 512 ? 256 : (n + 31) / 32 * 32;
-    const size_t smem = static_cast<size_t>((n + threads - 1) / threads) * threads * sizeof(T);
-    auto kernel = add_rms_norm_i8_kernel<T, 1, 0>;
+  if (VEC > 1 && n <= 256) {
+    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, (VEC > 1 ? 1 : 0)>, 1));
+  } else if (VEC > 1 && n <= 512) {
+    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, (VEC > 1 ? 2 : 0)>, 2));
+  } else if (VEC > 1 && n <= 2048) {
+    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, (VEC > 1 ? 4 : 0)>, 4));
+  } else {
+    const int threads = n >= 2048 ? 512 : n >= 512 ? 256 : (n + 31) / 32 * 32;
+    const size_t smem = static_cast<size_t>((n + threads - 1) / threads) * threads * VEC * sizeof(T);
+    auto kernel = add_rms_norm_i8_kernel<T, VEC, 0>;
     if (smem > 48 * 1024)
       DLM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          static_cast<int>(kNormMaxK * sizeof(T))));
+                                          static_cast<int>((kNormMaxK + 512) * sizeof(T))));
     DLM_CHECK_CUDA(launch_pdl(kernel, dim3(p.M), dim3(threads), smem, s, p));
-  } else if (n <= 256) {
-    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, 1>, 1));
-  } else if (n <= 512) {
-    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, 2>, 2));
-  } else if (n <= 2048) {
-    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, 4>, 4));
-  } else {
-    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, 8>, 8));
   }
   return DLM_OK;
 }
