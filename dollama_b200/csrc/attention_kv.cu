@@ -8,22 +8,27 @@
 // The g = Hq / Hkv heads of one kv head times the queries of one sequence are the rows of one
 // problem (row r: query r / g, head r % g), so a key is read once for all of them.
 //
-// One cluster of C CTAs takes 16 rows of one (sequence, kv head); its CTAs' warps take 32 keys at a
+// A cluster of C CTAs takes 8 NR rows of one (sequence, kv head); its CTAs' warps take 32 keys at a
 // time in turn, each with its own running maximum and sum (one pass over the cache), and the
 // partial results meet in shared memory: the warps' in their CTA, the CTAs' over the cluster, in a
-// fixed order.  Codes go from global memory straight into matrix-instruction fragments: which k
-// index of a fragment stands for which d (or key) is free as long as both operands agree, so a
-// lane takes 16 consecutive bytes of a key, and for V the same 8 (16) channels of four keys.  An
-// int8 code becomes an fp16 value exactly (0x6400 | (code + 128) is 1152 + code).  The scales stay
-// outside the products: kscale multiplies the finished dot product; vscale multiplies p in fp32.
+// fixed order.  A warp's keys arrive through its own ring of asynchronous copies (16-byte pieces
+// XORed with the row, so that both operands' reads are free of bank conflicts).
+//
+// Both products are transposed (keys, then channels, are the matrix instruction's 16 rows; the
+// queries its 8 columns), so that a few rows waste little, and their A operands come straight from
+// the codes: which k index of a fragment stands for which d (or key) is free as long as both
+// operands agree, so a lane takes 16 consecutive bytes of a key, and for V the same 8 (16) channels
+// of four keys.  An int8 code becomes an fp16 value exactly (0x6400 | (code + 128) is 1152 + code).
+// The scales stay outside the products: kscale multiplies the finished dot product; vscale
+// multiplies p in fp32.
 //
 // Precision: q is exact in fp16 for fp16, scaled per row by a power of two to [2^14, 2^15) for bf16
 // (exact down to 2^-25 of the row's maximum) and split into two fp16 terms for fp32.  The weights
 // w_ij = p_ij vscale_j are scaled by a power of two that follows the row's largest one, to [2^14,
 // 2^15), and rounded to fp16 (a relative error of 2^-11 each, down to 2^-29 of the largest), for
 // fp32 split into two terms; each row has its own scale, so a key that a row does not see has no
-// part in it.  Sums are fp32.
-#include <cfloat>
+// part in it.  The reference of p (a running maximum) and that scale move only when a score passes
+// it by 8 (p <= 2^8) or a weight would leave fp16.  Sums are fp32.
 #include <cstdint>
 
 #include "dtype.cuh"
@@ -35,8 +40,17 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 16;   // rows of one tile
-constexpr int kUnit = 32;   // keys a warp takes at a time
+constexpr int kUnit = 32;  // keys a warp takes at a time
+
+// NR: tiles of 8 rows
+template <int DH, int NR>
+struct Cfg {
+  static constexpr int kStages = DH == 64 ? 3 : 2;
+  static constexpr int kStage = kUnit * (2 * DH + 8);  // K, V codes, two scales
+  static constexpr int kWarpBytes = kStages * kStage;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+  static_assert(kWarpBytes >= 8 * NR * DH * 4, "a warp's partial result reuses its ring");
+};
 
 struct AttnKvParams {
   const void* q;
@@ -87,18 +101,39 @@ __device__ __forceinline__ float ld_dsmem(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-template <typename T, int DH>
+__device__ __forceinline__ void cp_async4(void* dst_smem, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst_smem)), "l"(src), "r"(bytes)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// byte of 16-byte piece `ch` of key row `r` in a staged [32][DH] block
+template <int DH>
+__device__ __forceinline__ int swz(int r, int ch) {
+  if constexpr (DH == 128) return r * 128 + ((ch ^ (r & 6) ^ ((r & 1) << 2)) << 4);
+  const int m = r >> 1;
+  return m * 128 + (((r ^ m) & 1) << 6) + ((ch ^ (m & 2)) << 4);
+}
+
+template <typename T, int DH, int NR>
 __global__ void __launch_bounds__(kThreads)
     attn_kv_kernel(const AttnKvParams p) {
-  constexpr bool kSplit = sizeof(T) == 4;                    // two fp16 terms for q and p
+  using C = Cfg<DH, NR>;
+  constexpr int kRows = 8 * NR;
+  constexpr bool kSplit = sizeof(T) == 4;                    // two fp16 terms for q and the weights
   constexpr bool kScaled = !std::is_same<T, __half>::value;  // q scaled into fp16's range
   constexpr int NT = kSplit ? 2 : 1;
-  constexpr int KS = DH / 16;   // k-steps of q.k
-  constexpr int DJ = DH / 8;    // channel tiles of p.v
+  constexpr int KS = DH / 16;  // k-steps of q.k, and channel tiles of p.v
+  constexpr int DJ = DH / 8;   // channels of a lane
   griddep_wait();  // inputs come from the previous kernel (programmatic dependent launch)
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   __shared__ float s_cm[kRows], s_cl[kRows];
-  extern __shared__ float s_o[];  // [kWarps][kRows][DH]
+  extern __shared__ __align__(128) uint8_t s_ring[];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, c4 = lane & 3;
@@ -119,25 +154,63 @@ __global__ void __launch_bounds__(kThreads)
   const int r0 = rt * kRows;
   // keys row r sees: [0, vis(r))
   auto vis = [&](int r) {
-    if (r >= rows) return 0;
     if (!p.causal) return n_kv;
     const int e = n_kv - n_q + r / p.g + 1;
     return e < 0 ? 0 : e;
   };
   const int last = (r0 + kRows < rows ? r0 + kRows : rows) - 1;
   const int n_keys = last < r0 ? 0 : vis(last);  // the last row sees the most
-  const int lim[2] = {vis(r0 + gr), vis(r0 + gr + 8)};
+  const int n_all = last < r0 ? 0 : vis(r0);     // keys that every row sees
+  int lim[NR][2];                                // of rows 2 c4 and 2 c4 + 1
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int r = r0 + 8 * n + 2 * c4 + z;
+      lim[n][z] = r <= last ? vis(r) : n_keys;
+    }
 
-  // ---- q fragments: rows gr and gr + 8, channels 16 c4 + 4 t + {0, 1 | 2, 3} (+ 64 from k-step 4 on)
-  uint32_t qf[NT][KS][4];
-  float qmul[2];
+  const size_t head = static_cast<size_t>(b) * p.Hkv + hkv;
+  const int8_t* kb = p.kq + head * p.Lmax * DH;
+  const int8_t* vb = p.vq + head * p.Lmax * DH;
+  const float* ksb = p.ks + head * p.Lmax;
+  const float* vsb = p.vs + head * p.Lmax;
+  uint8_t* ring = s_ring + warp * C::kWarpBytes;
+  const int stride = p.C * kWarps * kUnit;
+
+  // keys k0 .. k0 + 31 into stage st (zeros beyond n_keys)
+  auto fetch = [&](int k0, int st) {
+    if (k0 < n_keys) {
+      uint8_t* dst = ring + st * C::kStage;
+      constexpr int kPieces = DH / 16;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = (i * 32 + lane) / kPieces, ch = (i * 32 + lane) % kPieces;
+        const bool in = k0 + r < n_keys;
+        const size_t off = in ? static_cast<size_t>(k0 + r) * DH + ch * 16 : 0;
+        cp_async16(dst + swz<DH>(r, ch), kb + off, in ? 16u : 0u);
+        cp_async16(dst + kUnit * DH + swz<DH>(r, ch), vb + off, in ? 16u : 0u);
+      }
+      const bool in = k0 + lane < n_keys;
+      const size_t off = in ? k0 + lane : 0;
+      cp_async4(dst + 2 * kUnit * DH + 4 * lane, ksb + off, in ? 4u : 0u);
+      cp_async4(dst + 2 * kUnit * DH + 4 * (kUnit + lane), vsb + off, in ? 4u : 0u);
+    }
+    cp_async_commit();
+  };
+  int k_next = (rank * kWarps + warp) * kUnit;
+  for (int i = 0; i < C::kStages - 1; ++i, k_next += stride) fetch(k_next, i);
+
+  // ---- q, the B operand: row gr, channels 64 h + 16 c4 + 4 z + {0, 1 | 2, 3} in k-step 4 h + z
+  uint32_t qf[NT][NR][KS][2];
+  float qmul[NR][2];  // of rows 2 c4 and 2 c4 + 1
   {
     const T* q = static_cast<const T*>(p.q);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = r0 + gr + 8 * h;
+    for (int n = 0; n < NR; ++n) {
+      const int r = r0 + 8 * n + gr;
       float f[KS * 4];
-      if (r < rows) {
+      if (r <= last) {
         const T* src = q + (static_cast<size_t>(b) * p.Sq + r / p.g) * p.ldq +
                        (static_cast<size_t>(hkv) * p.g + r % p.g) * DH;
 #pragma unroll
@@ -146,223 +219,253 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int i = 0; i < KS * 4; ++i) f[i] = 0.0f;
       }
-      float up = 1.0f;
-      qmul[h] = p.scale_log2;
+      float up = 1.0f, mul = p.scale_log2;
       if constexpr (kScaled) {
         float mx = 0.0f;
 #pragma unroll
         for (int i = 0; i < KS * 4; ++i) mx = fmaxf(mx, fabsf(f[i]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        int e = 15 - exp_above(mx);
-        e = e > 100 ? 100 : e;  // rows below 2^-85: products below 2^-78 of any use
+        const int e = min(15 - exp_above(mx), 100);  // (rows below 2^-85 score 0)
         up = pow2i(e);
-        qmul[h] = p.scale_log2 * pow2i(-e);
+        mul = p.scale_log2 * pow2i(-e);
       }
+      qmul[n][0] = __shfl_sync(0xffffffffu, mul, 8 * c4);  // lane 4 r holds row r
+      qmul[n][1] = __shfl_sync(0xffffffffu, mul, 8 * c4 + 4);
 #pragma unroll
       for (int i = 0; i < KS * 2; ++i) {
         const float a0 = f[2 * i] * up, a1 = f[2 * i + 1] * up;
         const __half2 hi = __floats2half2_rn(a0, a1);
-        qf[0][i >> 1][(i & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&hi);
+        qf[0][n][i >> 1][i & 1] = *reinterpret_cast<const uint32_t*>(&hi);
         if constexpr (kSplit) {
           const float2 hf = __half22float2(hi);
           const __half2 lo = __floats2half2_rn(a0 - hf.x, a1 - hf.y);
-          qf[NT - 1][i >> 1][(i & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&lo);
+          qf[NT - 1][n][i >> 1][i & 1] = *reinterpret_cast<const uint32_t*>(&lo);
         }
       }
     }
   }
 
-  const size_t head = static_cast<size_t>(b) * p.Hkv + hkv;
-  const int8_t* kb = p.kq + head * p.Lmax * DH;
-  const int8_t* vb = p.vq + head * p.Lmax * DH;
-  const float* ksb = p.ks + head * p.Lmax;
-  const float* vsb = p.vs + head * p.Lmax;
-
-  float o[DJ][4];
+  // o: channels gr * DJ + 2 j + {0: [0..1], 1: [2..3]} of rows 2 c4 + {0, 1}, times 2^(15 - ew)
+  float o[NR][KS][4];
+  float m[NR][2], l[NR][2], up[NR][2];
+  int ew[NR][2];
 #pragma unroll
-  for (int j = 0; j < DJ; ++j)
+  for (int n = 0; n < NR; ++n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[j][i] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  // largest |weight| of each row so far (relative to m) and its exponent: o is sum w code 2^(15 - ew)
-  float wm[2] = {0.0f, 0.0f};
-  int ew[2] = {-100, -100};
-
-  for (int k0 = (rank * kWarps + warp) * kUnit; k0 < n_keys; k0 += p.C * kWarps * kUnit) {
-    // ---- loads: K codes of key 8 i + gr, V codes of keys 16 u + {2 c4, + 1, + 8, + 9}, scales
-    uint4 kw[4][DH / 64];
-    Vec<uint32_t, DH / 32> vw[2][4];
-    float ksc[4][2], vsc[4][2];
+    for (int j = 0; j < KS; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = k0 + 8 * i + gr;
+      for (int i = 0; i < 4; ++i) o[n][j][i] = 0.0f;
 #pragma unroll
-      for (int h = 0; h < DH / 64; ++h)
-        kw[i][h] = key < n_keys ? *reinterpret_cast<const uint4*>(kb + static_cast<size_t>(key) * DH + h * 64 + 16 * c4)
-                                : make_uint4(0, 0, 0, 0);
+    for (int z = 0; z < 2; ++z) {
+      m[n][z] = -1e30f;
+      l[n][z] = 0.0f;
+      ew[n][z] = -100;
+      up[n][z] = pow2i(115);
     }
+  }
+
+  int st = 0;
+  for (int k0 = (rank * kWarps + warp) * kUnit; k0 < n_keys; k0 += stride, k_next += stride) {
+    fetch(k_next, st == 0 ? C::kStages - 1 : st - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+    __syncwarp();
+    const uint8_t* sk = ring + st * C::kStage;
+    const uint8_t* sv = sk + kUnit * DH;
+    const float* sks = reinterpret_cast<const float*>(sv + kUnit * DH);
+    // ---- scores: keys 16 t + gr + {0: [0..1], 8: [2..3]} of rows 2 c4 + {0, 1}
+    float s[2][NR][4];
+    float ksc[2][2], vsc[2][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int key = k0 + 8 * i + 2 * c4 + h;
-        const bool in = key < n_keys;
-        ksc[i][h] = in ? ksb[key] : 0.0f;
-        vsc[i][h] = in ? vsb[key] : 0.0f;
-      }
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = k0 + 16 * u + 2 * c4 + (i >> 1) * 8 + (i & 1);
-        if (key < n_keys) {
-          vw[u][i] = *reinterpret_cast<const Vec<uint32_t, DH / 32>*>(vb + static_cast<size_t>(key) * DH + gr * DJ);
-        } else {
-#pragma unroll
-          for (int z = 0; z < DH / 32; ++z) vw[u][i].v[z] = 0;
-        }
-      }
-    // ---- scores
-    float s[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) s[u][n][j] = 0.0f;
 #pragma unroll
       for (int h = 0; h < DH / 64; ++h) {
-        const uint32_t w[4] = {kw[i][h].x, kw[i][h].y, kw[i][h].z, kw[i][h].w};
+        const uint4 w0 = *reinterpret_cast<const uint4*>(sk + swz<DH>(16 * u + gr, 4 * h + c4));
+        const uint4 w1 = *reinterpret_cast<const uint4*>(sk + swz<DH>(16 * u + gr + 8, 4 * h + c4));
+        const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
-          const uint32_t x = w[z] ^ 0x80808080u;
-          const uint32_t b0 = code_pair(x, 0x4140), b1 = code_pair(x, 0x4342);
+          const uint32_t y0 = x0[z] ^ 0x80808080u, y1 = x1[z] ^ 0x80808080u;
+          const uint32_t a[4] = {code_pair(y0, 0x4140), code_pair(y1, 0x4140), code_pair(y0, 0x4342),
+                                 code_pair(y1, 0x4342)};
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(s[i], qf[n][h * 4 + z], b0, b1);
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int k = 0; k < NT; ++k) mma_f16(s[u][n], a, qf[k][n][4 * h + z][0], qf[k][n][4 * h + z][1]);
         }
       }
-    }
-    float mx[2] = {m[0], m[1]};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = k0 + 8 * i + 2 * c4 + (j & 1);
-        s[i][j] = key < lim[j >> 1] ? s[i][j] * (ksc[i][j & 1] * qmul[j >> 1]) : -INFINITY;
-        mx[j >> 1] = fmaxf(mx[j >> 1], s[i][j]);
-      }
-#pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-      mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], x));
-      mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], x));
-    }
-    // ---- weights: s becomes w
-    float alpha[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float mu = mx[h] == -INFINITY ? 0.0f : mx[h];  // no visible key yet
-      alpha[h] = fast_exp2(m[h] - mu);
-      m[h] = mx[h];
-      l[h] *= alpha[h];
-      wm[h] *= alpha[h];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int key = k0 + 8 * i + 2 * c4 + z;
-          const float e = fast_exp2(s[i][2 * h + z] - mu);
-          l[h] += e;
-          // a masked key's scale may be anything
-          s[i][2 * h + z] = key < lim[h] ? e * vsc[i][z] : 0.0f;
-          wm[h] = fmaxf(wm[h], fabsf(s[i][2 * h + z]));
-        }
-    }
-#pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
-      wm[0] = fmaxf(wm[0], __shfl_xor_sync(0xffffffffu, wm[0], x));
-      wm[1] = fmaxf(wm[1], __shfl_xor_sync(0xffffffffu, wm[1], x));
-    }
-    float up[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = max(exp_above(wm[h]), -100);
-      const float a = alpha[h] * pow2i(min(max(ew[h] - e, -126), 127));
-      ew[h] = e;
-      up[h] = pow2i(15 - e);
-#pragma unroll
-      for (int j = 0; j < DJ; ++j) {
-        o[j][2 * h] *= a;
-        o[j][2 * h + 1] *= a;
-      }
-    }
-    // ---- the A operand of p.v: k-step u takes key tiles 2 u and 2 u + 1
-    uint32_t pf[NT][2][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float w0 = s[i][2 * h] * up[h], w1 = s[i][2 * h + 1] * up[h];
-        const __half2 hi = __floats2half2_rn(w0, w1);
-        pf[0][i >> 1][(i & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&hi);
-        if constexpr (kSplit) {
-          const float2 hf = __half22float2(hi);
-          const __half2 lo = __floats2half2_rn(w0 - hf.x, w1 - hf.y);
-          pf[NT - 1][i >> 1][(i & 1) * 2 + h] = *reinterpret_cast<const uint32_t*>(&lo);
-        }
+        ksc[u][h] = sks[16 * u + gr + 8 * h];
+        vsc[u][h] = sks[kUnit + 16 * u + gr + 8 * h];
       }
-    // ---- p.v
+    }
+    // s becomes the score relative to m, -inf for a key the row does not see
+    const bool masked = k0 + kUnit > n_all;
+    bool fits = true;
+    float w[2][NR][4], lu[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        float ls = 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& x = s[u][n][2 * h + z];
+            x = x * (ksc[u][h] * qmul[n][z]);
+            if (masked && k0 + 16 * u + gr + 8 * h >= lim[n][z]) x = -INFINITY;
+            const float d = x - m[n][z];
+            const float e = fast_exp2(d);
+            ls += e;
+            float y = e * (vsc[u][h] * up[n][z]);
+            if (masked && x == -INFINITY) y = 0.0f;  // a masked key's scale may be anything
+            w[u][n][2 * h + z] = y;
+            fits = fits && d <= 8.0f && fabsf(y) < 60000.0f;
+          }
+        lu[n][z] = l[n][z] + ls;
+      }
+    if (!__all_sync(0xffffffffu, fits)) {
+      // the references move (the first unit, a score well above the maximum so far, a large vscale)
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          float mx = m[n][z], ls = 0.0f;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mx = fmaxf(mx, s[u][n][2 * h + z]);
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          const float alpha = fast_exp2(m[n][z] - mx);
+          m[n][z] = mx;
+          float wm = 0.75f * pow2i(ew[n][z]) * alpha;  // about the largest weight so far
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x = s[u][n][2 * h + z];
+              const float e = fast_exp2(x - mx);
+              ls += e;
+              const float y = x == -INFINITY ? 0.0f : e * vsc[u][h];
+              w[u][n][2 * h + z] = y;
+              wm = fmaxf(wm, fabsf(y));
+            }
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, x));
+          const int e = min(max(exp_above(wm), -100), 127);
+          const float a = alpha * pow2i(min(max(ew[n][z] - e, -126), 127));
+          ew[n][z] = e;
+          up[n][z] = pow2i(15 - e);
+          lu[n][z] = l[n][z] * alpha + ls;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[u][n][2 * h + z] *= up[n][z];
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
+            o[n][j][z] *= a;
+            o[n][j][2 + z] *= a;
+          }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      l[n][0] = lu[n][0];
+      l[n][1] = lu[n][1];
+    }
+    // ---- the weights as the B operand of p.v: [key][row] tiles transposed to [row][key]
+    uint32_t pf[NT][NR][2][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int z = 0; z < DH / 32; ++z) {
-        const uint32_t w0 = vw[u][0].v[z] ^ 0x80808080u, w1 = vw[u][1].v[z] ^ 0x80808080u;
-        const uint32_t w2 = vw[u][2].v[z] ^ 0x80808080u, w3 = vw[u][3].v[z] ^ 0x80808080u;
-        const uint32_t lo01 = __byte_perm(w0, w1, 0x5140), hi01 = __byte_perm(w0, w1, 0x7362);
-        const uint32_t lo23 = __byte_perm(w2, w3, 0x5140), hi23 = __byte_perm(w2, w3, 0x7362);
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma_f16(o[4 * z + 0], pf[n][u], code_pair(lo01, 0x4140), code_pair(lo23, 0x4140));
-          mma_f16(o[4 * z + 1], pf[n][u], code_pair(lo01, 0x4342), code_pair(lo23, 0x4342));
-          mma_f16(o[4 * z + 2], pf[n][u], code_pair(hi01, 0x4140), code_pair(hi23, 0x4140));
-          mma_f16(o[4 * z + 3], pf[n][u], code_pair(hi01, 0x4342), code_pair(hi23, 0x4342));
+        for (int h = 0; h < 2; ++h) {
+          const float w0 = w[u][n][2 * h], w1 = w[u][n][2 * h + 1];
+          const __half2 hi = __floats2half2_rn(w0, w1);
+          pf[0][n][u][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
+          if constexpr (kSplit) {
+            const float2 hf = __half22float2(hi);
+            const __half2 lo = __floats2half2_rn(w0 - hf.x, w1 - hf.y);
+            pf[NT - 1][n][u][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&lo));
+          }
+        }
+    // ---- p.v: channels gr * DJ .. + DJ - 1 of keys 16 u + 2 c4 + {0, 1, 8, 9}
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      Vec<uint32_t, DJ / 4> vw[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * u + 2 * c4 + (i >> 1) * 8 + (i & 1);
+        vw[i] = *reinterpret_cast<const Vec<uint32_t, DJ / 4>*>(sv + swz<DH>(r, gr * DJ / 16) + (gr * DJ) % 16);
+      }
+#pragma unroll
+      for (int z = 0; z < DJ / 4; ++z) {
+        const uint32_t w0 = vw[0].v[z] ^ 0x80808080u, w1 = vw[1].v[z] ^ 0x80808080u;
+        const uint32_t w2 = vw[2].v[z] ^ 0x80808080u, w3 = vw[3].v[z] ^ 0x80808080u;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {  // channels 4 z + 2 y + {0, 1}
+          const uint32_t x01 = __byte_perm(w0, w1, y ? 0x7362 : 0x5140);
+          const uint32_t x23 = __byte_perm(w2, w3, y ? 0x7362 : 0x5140);
+          const uint32_t a[4] = {code_pair(x01, 0x4140), code_pair(x01, 0x4342), code_pair(x23, 0x4140),
+                                 code_pair(x23, 0x4342)};
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+#pragma unroll
+            for (int k = 0; k < NT; ++k) mma_f16(o[n][2 * z + y], a, pf[k][n][u][0], pf[k][n][u][1]);
         }
       }
-  }
-
-  // ---- this warp's partial results: maximum, sum, and o in true scale
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float down = pow2i(ew[h] - 15);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    const int r = gr + 8 * h;
-    if (c4 == 0) {
-      s_m[warp][r] = m[h];
-      s_l[warp][r] = l[h];
     }
-    float* dst = s_o + (warp * kRows + r) * DH;
-#pragma unroll
-    for (int z = 0; z < 2; ++z)
-#pragma unroll
-      for (int j = 0; j < DJ; ++j) dst[(2 * c4 + z) * DJ + j] = o[j][2 * h + z] * down;
+    if (++st == C::kStages) st = 0;
+    __syncwarp();  // every lane is done with the stage before its next fetch
   }
+  cp_async_wait_all();
+  __syncwarp();
+
+  // ---- this warp's partial results: maximum, sum, and o in true scale, into its ring
+  float* s_o = reinterpret_cast<float*>(ring);  // [kRows][DH]
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const float down = pow2i(ew[n][z] - 15);
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) l[n][z] += __shfl_xor_sync(0xffffffffu, l[n][z], x);
+      const int r = 8 * n + 2 * c4 + z;
+      if (gr == 0) {
+        s_m[warp][r] = m[n][z];
+        s_l[warp][r] = l[n][z];
+      }
+#pragma unroll
+      for (int j = 0; j < KS; j += 2)
+        *reinterpret_cast<float4*>(s_o + r * DH + gr * DJ + 2 * j) =
+            make_float4(o[n][j][z] * down, o[n][j][2 + z] * down, o[n][j + 1][z] * down, o[n][j + 1][2 + z] * down);
+    }
   __syncthreads();
-  // weight of a partial result with maximum m against the joint maximum M (0 where it saw no key)
-  auto weight = [](float mm, float M) { return mm == -INFINITY ? 0.0f : fast_exp2(mm - M); };
-  // ---- the CTA's warps join: thread covers channels of a row in turn
+  // ---- the CTA's warps join, element by element (each read and written by one thread)
+  s_o = reinterpret_cast<float*>(s_ring);
+  constexpr int kWarpFloats = C::kWarpBytes / 4;
   for (int i = threadIdx.x; i < kRows * DH; i += kThreads) {
-    const int r = i / DH, d = i % DH;
+    const int r = i / DH;
     float M = s_m[0][r];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[w][r]);
     float acc = 0.0f, ls = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = weight(s_m[w][r], M);
-      acc = fmaf(f, s_o[(w * kRows + r) * DH + d], acc);
+      const float f = fast_exp2(s_m[w][r] - M);
+      acc = fmaf(f, s_o[w * kWarpFloats + i], acc);
       ls = fmaf(f, s_l[w][r], ls);
     }
-    s_o[r * DH + d] = acc;  // this element of warp 0's block is read by this thread alone
-    if (d == 0) {
+    s_o[i] = acc;
+    if (i % DH == 0) {
       s_cm[r] = M;
       s_cl[r] = ls;
     }
@@ -389,7 +492,7 @@ __global__ void __launch_bounds__(kThreads)
     for (int c = 0; c < p.C; ++c) M = fmaxf(M, ld_dsmem(smem_u32(&s_cm[r]), c));
     float acc = 0.0f, L = 0.0f;
     for (int c = 0; c < p.C; ++c) {
-      const float f = weight(ld_dsmem(smem_u32(&s_cm[r]), c), M);
+      const float f = fast_exp2(ld_dsmem(smem_u32(&s_cm[r]), c) - M);
       acc = fmaf(f, ld_dsmem(smem_u32(&s_o[i]), c), acc);
       L = fmaf(f, ld_dsmem(smem_u32(&s_cl[r]), c), L);
     }
@@ -398,13 +501,41 @@ __global__ void __launch_bounds__(kThreads)
   cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
-template <typename T, int DH>
-int launch(const AttnKvParams& p, unsigned tiles, cudaStream_t s) {
-  constexpr int smem = kWarps * kRows * DH * 4;
+template <typename T, int DH, int NR>
+int launch(AttnKvParams p, cudaStream_t s) {
+  using C = Cfg<DH, NR>;
+  static int per_sm[64] = {0};  // CTAs an SM holds, by device
+  int dev = 0;
+  DLM_CHECK_CUDA(cudaGetDevice(&dev));
+  int resident = dev < 64 ? per_sm[dev] : 0;
+  if (resident == 0) {
+    DLM_CHECK_CUDA(cudaFuncSetAttribute(attn_kv_kernel<T, DH, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        C::kSmem));
+    DLM_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, attn_kv_kernel<T, DH, NR>, kThreads,
+                                                                 C::kSmem));
+    if (resident < 1) resident = 1;
+    if (dev < 64) per_sm[dev] = resident;
+  }
+  const long long row_tiles = (static_cast<long long>(p.Sq) * p.g + 8 * NR - 1) / (8 * NR);
+  const long long tiles = row_tiles * p.B * p.Hkv;
+  DLM_REQUIRE(tiles < (1ll << 27), DLM_ERR_UNSUPPORTED, "attention_kv_i8: too many rows");
+  p.row_tiles = static_cast<int>(row_tiles);
+  // CTAs per cluster: the size that needs the fewest waves for its share of the keys, as long as each
+  // warp has keys to take
+  const long long slots = static_cast<long long>(resident) * num_sms();
+  p.C = 1;
+  double best = 1e30;
+  for (int c = 1; c <= 8 && (c == 1 || (c - 1) * kWarps * kUnit < p.Lmax); ++c) {
+    const double cost = static_cast<double>((tiles * c + slots - 1) / slots) / c;
+    if (cost < 0.95 * best) {
+      best = cost;
+      p.C = c;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * p.C);
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.C));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -415,8 +546,16 @@ int launch(const AttnKvParams& p, unsigned tiles, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  DLM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_kv_kernel<T, DH>, p));
+  DLM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_kv_kernel<T, DH, NR>, p));
   return DLM_OK;
+}
+
+template <typename T, int DH>
+int launch_rows(const AttnKvParams& p, cudaStream_t s) {
+  const long long rows = static_cast<long long>(p.Sq) * p.g;
+  if (rows <= 8) return launch<T, DH, 1>(p, s);
+  if (rows <= 16 || DH == 128) return launch<T, DH, 2>(p, s);
+  return launch<T, DH, 4>(p, s);
 }
 
 }  // namespace
@@ -447,18 +586,12 @@ extern "C" int dlm_attention_kv_i8(const void* q, int ldq, const int8_t* kq, con
               "attention_kv_i8: cache codes must be 16-byte aligned");
   DLM_REQUIRE(scale > -INFINITY && scale < INFINITY, DLM_ERR_INVALID, "attention_kv_i8: scale is not finite");
   const int g = Hq / Hkv;
-  const long long row_tiles = (static_cast<long long>(Sq) * g + kRows - 1) / kRows;
-  const long long tiles = row_tiles * B * Hkv;
-  DLM_REQUIRE(tiles < (1ll << 27) && static_cast<long long>(Sq) * g < (1ll << 30), DLM_ERR_UNSUPPORTED,
-              "attention_kv_i8: too many rows");
-  // CTAs per cluster: enough to fill the SMs twice, as long as each warp has keys to take
-  int C = 1;
-  while (C < 8 && tiles * C < 2ll * num_sms() && 2ll * C * kWarps * kUnit <= Lmax) C *= 2;
-  AttnKvParams p{q, kq, kscale, vq, vscale, out, kv_len, q_len, ldq, ldo, B, Hq, Hkv, Sq, Lmax, g,
-                 static_cast<int>(row_tiles), causal, C, scale * 1.4426950408889634f, device_status_ptr()};
+  DLM_REQUIRE(static_cast<long long>(Sq) * g < (1ll << 30), DLM_ERR_UNSUPPORTED, "attention_kv_i8: too many rows");
+  const AttnKvParams p{q, kq, kscale, vq, vscale, out, kv_len, q_len, ldq, ldo, B, Hq, Hkv, Sq, Lmax, g,
+                       1, causal, 1, scale * 1.4426950408889634f, device_status_ptr()};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DLM_DISPATCH_DTYPE(dtype, T, {
-    if (Dh == 64) return launch<T, 64>(p, static_cast<unsigned>(tiles), s);
-    return launch<T, 128>(p, static_cast<unsigned>(tiles), s);
+    if (Dh == 64) return launch_rows<T, 64>(p, s);
+    return launch_rows<T, 128>(p, s);
   });
 }
