@@ -178,18 +178,33 @@ __global__ void __launch_bounds__(kThreads)
   uint8_t* ring = s_ring + warp * C::kWarpBytes;
   const int stride = p.C * kWarps * kUnit;
 
-  // keys k0 .. k0 + 31 into stage st (zeros beyond n_keys)
+  // keys k0 .. k0 + 31 into stage st (zeros beyond n_keys): piece i * 32 + lane is bytes 16 lane ..
+  // of rows i * kRowsPer .., and its place repeats every 8 rows
+  constexpr int kPieces = DH / 16, kRowsPer = 32 / kPieces, kPeriod = 8 / kRowsPer;
+  int dst_off[kPeriod];
+#pragma unroll
+  for (int i = 0; i < kPeriod; ++i) dst_off[i] = swz<DH>(i * kRowsPer + lane / kPieces, lane % kPieces);
   auto fetch = [&](int k0, int st) {
-    if (k0 < n_keys) {
-      uint8_t* dst = ring + st * C::kStage;
-      constexpr int kPieces = DH / 16;
+    uint8_t* dst = ring + st * C::kStage;
+    if (k0 + kUnit <= n_keys) {
+      const int8_t* k = kb + static_cast<size_t>(k0) * DH + 16 * lane;
+      const int8_t* v = vb + static_cast<size_t>(k0) * DH + 16 * lane;
 #pragma unroll
       for (int i = 0; i < kPieces; ++i) {
-        const int r = (i * 32 + lane) / kPieces, ch = (i * 32 + lane) % kPieces;
-        const bool in = k0 + r < n_keys;
-        const size_t off = in ? static_cast<size_t>(k0 + r) * DH + ch * 16 : 0;
-        cp_async16(dst + swz<DH>(r, ch), kb + off, in ? 16u : 0u);
-        cp_async16(dst + kUnit * DH + swz<DH>(r, ch), vb + off, in ? 16u : 0u);
+        uint8_t* d = dst + dst_off[i % kPeriod] + (i / kPeriod) * 8 * DH;
+        cp_async16(d, k + i * 512, 16);
+        cp_async16(d + kUnit * DH, v + i * 512, 16);
+      }
+      cp_async4(dst + 2 * kUnit * DH + 4 * lane, ksb + k0 + lane, 4);
+      cp_async4(dst + 2 * kUnit * DH + 4 * (kUnit + lane), vsb + k0 + lane, 4);
+    } else if (k0 < n_keys) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const bool in = k0 + i * kRowsPer + lane / kPieces < n_keys;
+        const size_t off = in ? static_cast<size_t>(k0) * DH + i * 512 + 16 * lane : 0;
+        uint8_t* d = dst + dst_off[i % kPeriod] + (i / kPeriod) * 8 * DH;
+        cp_async16(d, kb + off, in ? 16u : 0u);
+        cp_async16(d + kUnit * DH, vb + off, in ? 16u : 0u);
       }
       const bool in = k0 + lane < n_keys;
       const size_t off = in ? k0 + lane : 0;
@@ -265,14 +280,21 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
 
+  // this lane's pieces: key row gr, channels 64 h + 16 c4; value rows 2 c4 and 2 c4 + 1, channels
+  // gr * DJ (the places repeat every 8 rows)
+  int k_off[DH / 64], v_off[2];
+#pragma unroll
+  for (int h = 0; h < DH / 64; ++h) k_off[h] = swz<DH>(gr, 4 * h + c4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v_off[i] = kUnit * DH + swz<DH>(2 * c4 + i, gr * DJ / 16) + (gr * DJ) % 16;
+
   int st = 0;
   for (int k0 = (rank * kWarps + warp) * kUnit; k0 < n_keys; k0 += stride, k_next += stride) {
     fetch(k_next, st == 0 ? C::kStages - 1 : st - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
     __syncwarp();
     const uint8_t* sk = ring + st * C::kStage;
-    const uint8_t* sv = sk + kUnit * DH;
-    const float* sks = reinterpret_cast<const float*>(sv + kUnit * DH);
+    const float* sks = reinterpret_cast<const float*>(sk + 2 * kUnit * DH) + gr;
     // ---- scores: keys 16 t + gr + {0: [0..1], 8: [2..3]} of rows 2 c4 + {0, 1}
     float s[2][NR][4];
     float ksc[2][2], vsc[2][2];
@@ -284,8 +306,8 @@ __global__ void __launch_bounds__(kThreads)
         for (int j = 0; j < 4; ++j) s[u][n][j] = 0.0f;
 #pragma unroll
       for (int h = 0; h < DH / 64; ++h) {
-        const uint4 w0 = *reinterpret_cast<const uint4*>(sk + swz<DH>(16 * u + gr, 4 * h + c4));
-        const uint4 w1 = *reinterpret_cast<const uint4*>(sk + swz<DH>(16 * u + gr + 8, 4 * h + c4));
+        const uint4 w0 = *reinterpret_cast<const uint4*>(sk + k_off[h] + 16 * u * DH);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(sk + k_off[h] + (16 * u + 8) * DH);
         const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
@@ -300,37 +322,41 @@ __global__ void __launch_bounds__(kThreads)
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ksc[u][h] = sks[16 * u + gr + 8 * h];
-        vsc[u][h] = sks[kUnit + 16 * u + gr + 8 * h];
+        ksc[u][h] = sks[16 * u + 8 * h];
+        vsc[u][h] = sks[kUnit + 16 * u + 8 * h];
       }
     }
-    // s becomes the score relative to m, -inf for a key the row does not see
+    // weights against the references so far (a masked key's scale may be anything)
     const bool masked = k0 + kUnit > n_all;
-    bool fits = true;
-    float w[2][NR][4], lu[NR][2];
+    float w[2][NR][4], lu[NR][2], top = -INFINITY, big = 0.0f;
+    auto weigh = [&](auto mask) {
 #pragma unroll
-    for (int n = 0; n < NR; ++n)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        float ls = 0.0f;
+        for (int z = 0; z < 2; ++z) {
+          lu[n][z] = l[n][z];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float& x = s[u][n][2 * h + z];
-            x = x * (ksc[u][h] * qmul[n][z]);
-            if (masked && k0 + 16 * u + gr + 8 * h >= lim[n][z]) x = -INFINITY;
-            const float d = x - m[n][z];
-            const float e = fast_exp2(d);
-            ls += e;
-            float y = e * (vsc[u][h] * up[n][z]);
-            if (masked && x == -INFINITY) y = 0.0f;  // a masked key's scale may be anything
-            w[u][n][2 * h + z] = y;
-            fits = fits && d <= 8.0f && fabsf(y) < 60000.0f;
+            for (int h = 0; h < 2; ++h) {
+              const int i = 2 * h + z;
+              float d = fmaf(s[u][n][i], ksc[u][h] * qmul[n][z], -m[n][z]);
+              const bool hidden = mask && k0 + 16 * u + gr + 8 * h >= lim[n][z];
+              if (hidden) d = -INFINITY;
+              const float e = fast_exp2(d);
+              lu[n][z] += e;
+              w[u][n][i] = hidden ? 0.0f : e * (vsc[u][h] * up[n][z]);
+              top = fmaxf(top, d);
+            }
+            big = max3f(big, fabsf(w[u][n][z]), fabsf(w[u][n][2 + z]));
           }
-        lu[n][z] = l[n][z] + ls;
-      }
-    if (!__all_sync(0xffffffffu, fits)) {
+        }
+    };
+    if (masked)
+      weigh(std::true_type{});
+    else
+      weigh(std::false_type{});
+    if (__any_sync(0xffffffffu, top > 8.0f || big >= 60000.0f)) {
       // the references move (the first unit, a score well above the maximum so far, a large vscale)
 #pragma unroll
       for (int n = 0; n < NR; ++n)
@@ -340,7 +366,12 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) mx = fmaxf(mx, s[u][n][2 * h + z]);
+            for (int h = 0; h < 2; ++h) {
+              float& x = s[u][n][2 * h + z];
+              x *= ksc[u][h] * qmul[n][z];
+              if (k0 + 16 * u + gr + 8 * h >= lim[n][z]) x = -INFINITY;
+              mx = fmaxf(mx, x);
+            }
 #pragma unroll
           for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
           const float alpha = fast_exp2(m[n][z] - mx);
@@ -353,7 +384,7 @@ __global__ void __launch_bounds__(kThreads)
               const float x = s[u][n][2 * h + z];
               const float e = fast_exp2(x - mx);
               ls += e;
-              const float y = x == -INFINITY ? 0.0f : e * vsc[u][h];
+              const float y = k0 + 16 * u + gr + 8 * h >= lim[n][z] ? 0.0f : e * vsc[u][h];
               w[u][n][2 * h + z] = y;
               wm = fmaxf(wm, fabsf(y));
             }
@@ -403,8 +434,8 @@ __global__ void __launch_bounds__(kThreads)
       Vec<uint32_t, DJ / 4> vw[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = 16 * u + 2 * c4 + (i >> 1) * 8 + (i & 1);
-        vw[i] = *reinterpret_cast<const Vec<uint32_t, DJ / 4>*>(sv + swz<DH>(r, gr * DJ / 16) + (gr * DJ) % 16);
+        const uint8_t* src = sk + v_off[i & 1] + (16 * u + (i >> 1) * 8) * DH;
+        vw[i] = *reinterpret_cast<const Vec<uint32_t, DJ / 4>*>(src);
       }
 #pragma unroll
       for (int z = 0; z < DJ / 4; ++z) {
