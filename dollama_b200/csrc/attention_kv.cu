@@ -62,7 +62,7 @@ struct AttnKvParams {
   const int* kv_len;
   const int* q_len;
   long long ldq, ldo;
-  int B, Hq, Hkv, Sq, Lmax, g, row_tiles, causal, C;
+  int B, Hq, Hkv, Sq, Lmax, g, row_tiles, tiles, causal, C;
   float scale_log2;
   int* status;
 };
@@ -120,7 +120,7 @@ __device__ __forceinline__ int swz(int r, int ch) {
   return m * 128 + (((r ^ m) & 1) << 6) + ((ch ^ (m & 2)) << 4);
 }
 
-template <typename T, int DH, int NR>
+template <typename T, int DH, int NR, bool kSolo>
 __global__ void __launch_bounds__(kThreads)
     attn_kv_kernel(const AttnKvParams p) {
   using C = Cfg<DH, NR>;
@@ -137,15 +137,16 @@ __global__ void __launch_bounds__(kThreads)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, c4 = lane & 3;
-  const int rank = static_cast<int>(blockIdx.x % p.C);
-  int t = static_cast<int>(blockIdx.x / p.C);
+  const int rank = kSolo ? 0 : static_cast<int>(blockIdx.x % p.C);
+  int t = kSolo ? static_cast<int>(blockIdx.x) * kWarps + warp : static_cast<int>(blockIdx.x / p.C);
+  if (kSolo && t >= p.tiles) return;  // (a lone warp meets no barrier)
   const int rt = t % p.row_tiles;
   t /= p.row_tiles;
   const int hkv = t % p.Hkv, b = t / p.Hkv;
 
   int n_kv = p.kv_len[b];
   if (n_kv < 0 || n_kv > p.Lmax) {
-    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, kDevBadPosition);
+    if ((kSolo ? lane : threadIdx.x) == 0 && p.status) atomicCAS(p.status, 0, kDevBadPosition);
     n_kv = n_kv < 0 ? 0 : p.Lmax;
   }
   int n_q = p.q_len ? p.q_len[b] : p.Sq;
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kThreads)
   const float* ksb = p.ks + head * p.Lmax;
   const float* vsb = p.vs + head * p.Lmax;
   uint8_t* ring = s_ring + warp * C::kWarpBytes;
-  const int stride = p.C * kWarps * kUnit;
+  const int first = kSolo ? 0 : (rank * kWarps + warp) * kUnit, stride = kSolo ? kUnit : p.C * kWarps * kUnit;
 
   // keys k0 .. k0 + 31 into stage st (zeros beyond n_keys): piece i * 32 + lane is bytes 16 lane ..
   // of rows i * kRowsPer .., and its place repeats every 8 rows
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     cp_async_commit();
   };
-  int k_next = (rank * kWarps + warp) * kUnit;
+  int k_next = first;
   for (int i = 0; i < C::kStages - 1; ++i, k_next += stride) fetch(k_next, i);
 
   // ---- q, the B operand: row gr, channels 64 h + 16 c4 + 4 z + {0, 1 | 2, 3} in k-step 4 h + z
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kThreads)
   for (int i = 0; i < 2; ++i) v_off[i] = kUnit * DH + swz<DH>(2 * c4 + i, gr * DJ / 16) + (gr * DJ) % 16;
 
   int st = 0;
-  for (int k0 = (rank * kWarps + warp) * kUnit; k0 < n_keys; k0 += stride, k_next += stride) {
+  for (int k0 = first; k0 < n_keys; k0 += stride, k_next += stride) {
     fetch(k_next, st == 0 ? C::kStages - 1 : st - 1);
     asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
     __syncwarp();
@@ -460,6 +461,35 @@ __global__ void __launch_bounds__(kThreads)
   cp_async_wait_all();
   __syncwarp();
 
+  T* out = static_cast<T*>(p.out);
+  auto out_row = [&](int r) {
+    const int row = r0 + r;
+    return out + (static_cast<size_t>(b) * p.Sq + row / p.g) * p.ldo +
+           (static_cast<size_t>(hkv) * p.g + row % p.g) * DH;
+  };
+  if constexpr (kSolo) {
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) l[n][z] += __shfl_xor_sync(0xffffffffu, l[n][z], x);
+        const int r = 8 * n + 2 * c4 + z;
+        if (r0 + r > last) continue;
+        const float down = l[n][z] == 0.0f ? 0.0f : pow2i(ew[n][z] - 15) / l[n][z];
+        constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+        Vec<T, kPer> v[DJ / kPer];
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+          v[2 * j / kPer].v[2 * j % kPer] = from_f<T>(o[n][j][z] * down);
+          v[(2 * j + 1) / kPer].v[(2 * j + 1) % kPer] = from_f<T>(o[n][j][2 + z] * down);
+        }
+        T* dst = out_row(r) + gr * DJ;
+#pragma unroll
+        for (int j = 0; j < DJ / kPer; ++j) reinterpret_cast<Vec<T, kPer>*>(dst)[j] = v[j];
+      }
+    return;
+  }
   // ---- this warp's partial results: maximum, sum, and o in true scale, into its ring
   float* s_o = reinterpret_cast<float*>(ring);  // [kRows][DH]
 #pragma unroll
@@ -501,12 +531,7 @@ __global__ void __launch_bounds__(kThreads)
       s_cl[r] = ls;
     }
   }
-  T* out = static_cast<T*>(p.out);
-  auto store = [&](int r, int d, float v) {
-    const int row = r0 + r;
-    out[(static_cast<size_t>(b) * p.Sq + row / p.g) * p.ldo + (static_cast<size_t>(hkv) * p.g + row % p.g) * DH +
-        d] = from_f<T>(v);
-  };
+  auto store = [&](int r, int d, float v) { out_row(r)[d] = from_f<T>(v); };
   const int n_rows = last - r0 + 1;  // rows of this tile that exist
   if (p.C == 1) {
     __syncthreads();
@@ -532,36 +557,54 @@ __global__ void __launch_bounds__(kThreads)
   cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
+// Raises the kernel's shared-memory limit and finds how many CTAs an SM holds, once per device.
+template <typename K>
+int residency(K kernel, int smem, int (&cache)[64], int& per_sm) {
+  int dev = 0;
+  DLM_CHECK_CUDA(cudaGetDevice(&dev));
+  per_sm = dev < 64 ? cache[dev] : 0;
+  if (per_sm > 0) return DLM_OK;
+  DLM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  DLM_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, smem));
+  if (per_sm < 1) per_sm = 1;
+  if (dev < 64) cache[dev] = per_sm;
+  return DLM_OK;
+}
+
 template <typename T, int DH, int NR>
 int launch(AttnKvParams p, cudaStream_t s) {
   using C = Cfg<DH, NR>;
-  static int per_sm[64] = {0};  // CTAs an SM holds, by device
-  int dev = 0;
-  DLM_CHECK_CUDA(cudaGetDevice(&dev));
-  int resident = dev < 64 ? per_sm[dev] : 0;
-  if (resident == 0) {
-    DLM_CHECK_CUDA(cudaFuncSetAttribute(attn_kv_kernel<T, DH, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        C::kSmem));
-    DLM_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, attn_kv_kernel<T, DH, NR>, kThreads,
-                                                                 C::kSmem));
-    if (resident < 1) resident = 1;
-    if (dev < 64) per_sm[dev] = resident;
-  }
+  static int cache[2][64] = {{0}};
+  int per_sm = 0, per_sm_solo = 0;
+  int rc = residency(attn_kv_kernel<T, DH, NR, false>, C::kSmem, cache[0], per_sm);
+  if (rc == DLM_OK) rc = residency(attn_kv_kernel<T, DH, NR, true>, C::kSmem, cache[1], per_sm_solo);
+  if (rc != DLM_OK) return rc;
   const long long row_tiles = (static_cast<long long>(p.Sq) * p.g + 8 * NR - 1) / (8 * NR);
   const long long tiles = row_tiles * p.B * p.Hkv;
   DLM_REQUIRE(tiles < (1ll << 27), DLM_ERR_UNSUPPORTED, "attention_kv_i8: too many rows");
   p.row_tiles = static_cast<int>(row_tiles);
-  // CTAs per cluster: the size that needs the fewest waves for its share of the keys, as long as each
-  // warp has keys to take
-  const long long slots = static_cast<long long>(resident) * num_sms();
-  p.C = 1;
-  double best = 1e30;
-  for (int c = 1; c <= 8 && (c == 1 || (c - 1) * kWarps * kUnit < p.Lmax); ++c) {
-    const double cost = static_cast<double>((tiles * c + slots - 1) / slots) / c;
-    if (cost < 0.95 * best) {
-      best = cost;
+  p.tiles = static_cast<int>(tiles);
+  // Waves times keys of a warp (plus its fixed work, about as long as kFixed keys), for one warp per
+  // tile and for clusters of 1 to 8 CTAs per tile.
+  constexpr double kFixed = 100.0;
+  auto cost = [&](long long ctas, int resident, int warps) {
+    const long long slots = static_cast<long long>(resident) * num_sms();
+    const long long units = (p.Lmax + static_cast<long long>(kUnit) * warps - 1) / (kUnit * warps);
+    return static_cast<double>((ctas + slots - 1) / slots) * (static_cast<double>(units * kUnit) + kFixed);
+  };
+  double best = cost((tiles + kWarps - 1) / kWarps, per_sm_solo, 1);
+  p.C = 0;
+  for (int c = 1; c <= 8; ++c) {
+    const double t = cost(tiles * c, per_sm, c * kWarps);
+    if (t < 0.97 * best) {
+      best = t;
       p.C = c;
     }
+  }
+  if (p.C == 0) {
+    DLM_CHECK_CUDA(launch_pdl(attn_kv_kernel<T, DH, NR, true>, dim3(static_cast<unsigned>((tiles + kWarps - 1) / kWarps)),
+                              dim3(kThreads), C::kSmem, s, p));
+    return DLM_OK;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.C));
@@ -577,7 +620,7 @@ int launch(AttnKvParams p, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  DLM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_kv_kernel<T, DH, NR>, p));
+  DLM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_kv_kernel<T, DH, NR, false>, p));
   return DLM_OK;
 }
 
@@ -585,8 +628,7 @@ template <typename T, int DH>
 int launch_rows(const AttnKvParams& p, cudaStream_t s) {
   const long long rows = static_cast<long long>(p.Sq) * p.g;
   if (rows <= 8) return launch<T, DH, 1>(p, s);
-  if (rows <= 16 || DH == 128) return launch<T, DH, 2>(p, s);
-  return launch<T, DH, 4>(p, s);
+  return launch<T, DH, 2>(p, s);
 }
 
 }  // namespace
@@ -619,7 +661,7 @@ extern "C" int dlm_attention_kv_i8(const void* q, int ldq, const int8_t* kq, con
   const int g = Hq / Hkv;
   DLM_REQUIRE(static_cast<long long>(Sq) * g < (1ll << 30), DLM_ERR_UNSUPPORTED, "attention_kv_i8: too many rows");
   const AttnKvParams p{q, kq, kscale, vq, vscale, out, kv_len, q_len, ldq, ldo, B, Hq, Hkv, Sq, Lmax, g,
-                       1, causal, 1, scale * 1.4426950408889634f, device_status_ptr()};
+                       1, 1, causal, 1, scale * 1.4426950408889634f, device_status_ptr()};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DLM_DISPATCH_DTYPE(dtype, T, {
     if (Dh == 64) return launch_rows<T, 64>(p, s);
