@@ -24,15 +24,10 @@
 //
 // Precision: q is exact in fp16 for fp16, scaled per row by a power of two to [2^14, 2^15) for bf16
 // (exact down to 2^-25 of the row's maximum) and split into two fp16 terms for fp32.  The weights
-// w_ij = p_ij vscale_j are scaled by a power of two that follows the row's largest one, to [2^14,
-// 2^15), and rounded to fp16 (a relative error of 2^-11 each, down to 2^-29 of the largest), for
-// fp32 split into two terms; each row has its own scale, so a key that a row does not see has no
-// part in it.  The reference of p (a running maximum) and that scale move only when a score passes
-// it by 8 (p <= 2^8) or a weight would leave fp16.  Sums are fp32.
-#include <cstdint>
-
-#include "dtype.cuh"
-#include "ptx.cuh"
+// w_ij = p_ij vscale_j are taken against a reference of their row's own that keeps the largest near
+// 2^14 (so a key that a row does not see has no part in it) and rounded to fp16 (a relative error of
+// 2^-11 each), for fp32 split into two terms.  Sums are fp32.
+#include "attention_kv.cuh"
 
 namespace dlm {
 
@@ -52,53 +47,12 @@ struct Cfg {
   static_assert(kWarpBytes >= 8 * NR * DH * 4, "a warp's partial result reuses its ring");
 };
 
-struct AttnKvParams {
-  const void* q;
-  const int8_t* kq;
-  const float* ks;
-  const int8_t* vq;
-  const float* vs;
-  void* out;
-  const int* kv_len;
-  const int* q_len;
-  long long ldq, ldo;
-  int B, Hq, Hkv, Sq, Lmax, g, row_tiles, tiles, causal, C;
-  float scale_log2;
-  int* status;
-};
-
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t code_pair(uint32_t biased, uint32_t sel) {
-  // two biased codes (code + 128) picked by sel -> fp16 pair of the codes
-  const uint32_t h = __byte_perm(biased, 0x64646464u, sel);
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __float2half2_rn(1152.0f));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// 2^e as a float for -126 <= e <= 127
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-// smallest e with |x| < 2^e for a normal x (the biased exponent alone)
-__device__ __forceinline__ int exp_above(float x) { return static_cast<int>((__float_as_uint(x) >> 23) & 0xFF) - 126; }
-
-__device__ __forceinline__ float ld_dsmem(uint32_t addr, uint32_t rank) {
-  float v;
-  asm volatile(
-      "{\n"
-      ".reg .b32 ra;\n"
-      "mapa.shared::cluster.u32 ra, %1, %2;\n"
-      "ld.shared::cluster.f32 %0, [ra];\n"
-      "}\n"
-      : "=f"(v)
-      : "r"(addr), "r"(rank)
-      : "memory");
-  return v;
 }
 
 __device__ __forceinline__ void cp_async4(void* dst_smem, const void* src, uint32_t bytes) {
@@ -138,40 +92,20 @@ __global__ void __launch_bounds__(kThreads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, c4 = lane & 3;
   const int rank = kSolo ? 0 : static_cast<int>(blockIdx.x % p.C);
-  int t = kSolo ? static_cast<int>(blockIdx.x) * kWarps + warp : static_cast<int>(blockIdx.x / p.C);
+  const int t = kSolo ? static_cast<int>(blockIdx.x) * kWarps + warp : static_cast<int>(blockIdx.x / p.C);
   if (kSolo && t >= p.tiles) return;  // (a lone warp meets no barrier)
-  const int rt = t % p.row_tiles;
-  t /= p.row_tiles;
-  const int hkv = t % p.Hkv, b = t / p.Hkv;
-
-  int n_kv = p.kv_len[b];
-  if (n_kv < 0 || n_kv > p.Lmax) {
-    if ((kSolo ? lane : threadIdx.x) == 0 && p.status) atomicCAS(p.status, 0, kDevBadPosition);
-    n_kv = n_kv < 0 ? 0 : p.Lmax;
-  }
-  int n_q = p.q_len ? p.q_len[b] : p.Sq;
-  n_q = n_q < 0 ? 0 : (n_q > p.Sq ? p.Sq : n_q);
-  const int rows = n_q * p.g;  // rows of this (sequence, kv head)
-  const int r0 = rt * kRows;
-  // keys row r sees: [0, vis(r))
-  auto vis = [&](int r) {
-    if (!p.causal) return n_kv;
-    const int e = n_kv - n_q + r / p.g + 1;
-    return e < 0 ? 0 : e;
-  };
-  const int last = (r0 + kRows < rows ? r0 + kRows : rows) - 1;
-  const int n_keys = last < r0 ? 0 : vis(last);  // the last row sees the most
-  const int n_all = last < r0 ? 0 : vis(r0);     // keys that every row sees
+  const AttnKvTile tile(p, t, kRows, (kSolo ? lane : threadIdx.x) == 0);
+  const int r0 = tile.r0, last = tile.last, n_keys = tile.n_keys, n_all = tile.n_all;
   int lim[NR][2];                                // of rows 2 c4 and 2 c4 + 1
 #pragma unroll
   for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
       const int r = r0 + 8 * n + 2 * c4 + z;
-      lim[n][z] = r <= last ? vis(r) : n_keys;
+      lim[n][z] = r <= last ? tile.seen(p, r) : n_keys;
     }
 
-  const size_t head = static_cast<size_t>(b) * p.Hkv + hkv;
+  const size_t head = tile.head(p);
   const int8_t* kb = p.kq + head * p.Lmax * DH;
   const int8_t* vb = p.vq + head * p.Lmax * DH;
   const float* ksb = p.ks + head * p.Lmax;
@@ -221,14 +155,12 @@ __global__ void __launch_bounds__(kThreads)
   uint32_t qf[NT][NR][KS][2];
   float qmul[NR][2];  // of rows 2 c4 and 2 c4 + 1
   {
-    const T* q = static_cast<const T*>(p.q);
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       const int r = r0 + 8 * n + gr;
       float f[KS * 4];
       if (r <= last) {
-        const T* src = q + (static_cast<size_t>(b) * p.Sq + r / p.g) * p.ldq +
-                       (static_cast<size_t>(hkv) * p.g + r % p.g) * DH;
+        const T* src = tile.q_row<T>(p, r, DH);
 #pragma unroll
         for (int i = 0; i < KS * 4; ++i) f[i] = to_f(src[(i >> 4) * 64 + 16 * c4 + (i & 15)]);
       } else {
@@ -242,7 +174,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int i = 0; i < KS * 4; ++i) mx = fmaxf(mx, fabsf(f[i]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = min(15 - exp_above(mx), 100);  // (rows below 2^-85 score 0)
+        const int e = q_up(mx);
         up = pow2i(e);
         mul = p.scale_log2 * pow2i(-e);
       }
@@ -251,21 +183,14 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int i = 0; i < KS * 2; ++i) {
         const float a0 = f[2 * i] * up, a1 = f[2 * i + 1] * up;
-        const __half2 hi = __floats2half2_rn(a0, a1);
-        qf[0][n][i >> 1][i & 1] = *reinterpret_cast<const uint32_t*>(&hi);
-        if constexpr (kSplit) {
-          const float2 hf = __half22float2(hi);
-          const __half2 lo = __floats2half2_rn(a0 - hf.x, a1 - hf.y);
-          qf[NT - 1][n][i >> 1][i & 1] = *reinterpret_cast<const uint32_t*>(&lo);
-        }
+        qf[0][n][i >> 1][i & 1] = half_pair(a0, a1);
+        if constexpr (kSplit) qf[NT - 1][n][i >> 1][i & 1] = half_rest(qf[0][n][i >> 1][i & 1], a0, a1);
       }
     }
   }
 
-  // o: channels gr * DJ + 2 j + {0: [0..1], 1: [2..3]} of rows 2 c4 + {0, 1}, times 2^(15 - ew)
-  float o[NR][KS][4];
-  float m[NR][2], l[NR][2], up[NR][2];
-  int ew[NR][2];
+  // o: channels gr * DJ + 2 j + {0: [0..1], 1: [2..3]} of rows 2 c4 + {0, 1}
+  float o[NR][KS][4], ref[NR][2], l[NR][2];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
 #pragma unroll
@@ -274,10 +199,8 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = 0; i < 4; ++i) o[n][j][i] = 0.0f;
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-      m[n][z] = -1e30f;
+      ref[n][z] = kNoRef;
       l[n][z] = 0.0f;
-      ew[n][z] = -100;
-      up[n][z] = pow2i(115);
     }
   }
 
@@ -329,7 +252,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     // weights against the references so far (a masked key's scale may be anything)
     const bool masked = k0 + kUnit > n_all;
-    float w[2][NR][4], lu[NR][2], top = -INFINITY, big = 0.0f;
+    float w[2][NR][4], lu[NR][2], big = 0.0f, sum = 0.0f;
     auto weigh = [&](auto mask) {
 #pragma unroll
       for (int n = 0; n < NR; ++n)
@@ -341,29 +264,28 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int i = 2 * h + z;
-              float d = fmaf(s[u][n][i], ksc[u][h] * qmul[n][z], -m[n][z]);
               const bool hidden = mask && k0 + 16 * u + gr + 8 * h >= lim[n][z];
-              if (hidden) d = -INFINITY;
-              const float e = fast_exp2(d);
+              const float d = fmaf(s[u][n][i], ksc[u][h] * qmul[n][z], -ref[n][z]);
+              const float e = hidden ? 0.0f : fast_exp2(d);
               lu[n][z] += e;
-              w[u][n][i] = hidden ? 0.0f : e * (vsc[u][h] * up[n][z]);
-              top = fmaxf(top, d);
+              w[u][n][i] = hidden ? 0.0f : e * vsc[u][h];
             }
             big = max3f(big, fabsf(w[u][n][z]), fabsf(w[u][n][2 + z]));
           }
+          sum = fmaxf(sum, lu[n][z]);
         }
     };
     if (masked)
       weigh(std::true_type{});
     else
       weigh(std::false_type{});
-    if (__any_sync(0xffffffffu, top > 8.0f || big >= 60000.0f)) {
-      // the references move (the first unit, a score well above the maximum so far, a large vscale)
+    if (__any_sync(0xffffffffu, big >= kMaxWeight || sum >= kMaxSum)) {
+      // the references move (the first unit, a score well above those so far, a large vscale)
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          float mx = m[n][z], ls = 0.0f;
+          float top = -INFINITY, top_w = -INFINITY;
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -371,39 +293,30 @@ __global__ void __launch_bounds__(kThreads)
               float& x = s[u][n][2 * h + z];
               x *= ksc[u][h] * qmul[n][z];
               if (k0 + 16 * u + gr + 8 * h >= lim[n][z]) x = -INFINITY;
-              mx = fmaxf(mx, x);
+              top = fmaxf(top, x);
+              top_w = fmaxf(top_w, weight_log2(x, vsc[u][h]));
             }
 #pragma unroll
-          for (int x = 4; x <= 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-          const float alpha = fast_exp2(m[n][z] - mx);
-          m[n][z] = mx;
-          float wm = 0.75f * pow2i(ew[n][z]) * alpha;  // about the largest weight so far
+          for (int x = 4; x <= 16; x <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            top_w = fmaxf(top_w, __shfl_xor_sync(0xffffffffu, top_w, x));
+          }
+          const float to = new_ref(ref[n][z], top, top_w);
+          const float alpha = fast_exp2(ref[n][z] - to);
+          ref[n][z] = to;
+          lu[n][z] = l[n][z] * alpha;
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float x = s[u][n][2 * h + z];
-              const float e = fast_exp2(x - mx);
-              ls += e;
-              const float y = k0 + 16 * u + gr + 8 * h >= lim[n][z] ? 0.0f : e * vsc[u][h];
-              w[u][n][2 * h + z] = y;
-              wm = fmaxf(wm, fabsf(y));
+              const float e = fast_exp2(s[u][n][2 * h + z] - to);
+              lu[n][z] += e;
+              w[u][n][2 * h + z] = k0 + 16 * u + gr + 8 * h >= lim[n][z] ? 0.0f : e * vsc[u][h];
             }
 #pragma unroll
-          for (int x = 4; x <= 16; x <<= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, x));
-          const int e = min(max(exp_above(wm), -100), 127);
-          const float a = alpha * pow2i(min(max(ew[n][z] - e, -126), 127));
-          ew[n][z] = e;
-          up[n][z] = pow2i(15 - e);
-          lu[n][z] = l[n][z] * alpha + ls;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) w[u][n][2 * h + z] *= up[n][z];
-#pragma unroll
           for (int j = 0; j < KS; ++j) {
-            o[n][j][z] *= a;
-            o[n][j][2 + z] *= a;
+            o[n][j][z] *= alpha;
+            o[n][j][2 + z] *= alpha;
           }
         }
     }
@@ -421,13 +334,9 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float w0 = w[u][n][2 * h], w1 = w[u][n][2 * h + 1];
-          const __half2 hi = __floats2half2_rn(w0, w1);
-          pf[0][n][u][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hi));
-          if constexpr (kSplit) {
-            const float2 hf = __half22float2(hi);
-            const __half2 lo = __floats2half2_rn(w0 - hf.x, w1 - hf.y);
-            pf[NT - 1][n][u][h] = transpose8x8(*reinterpret_cast<const uint32_t*>(&lo));
-          }
+          const uint32_t hi = half_pair(w0, w1);
+          pf[0][n][u][h] = transpose8x8(hi);
+          if constexpr (kSplit) pf[NT - 1][n][u][h] = transpose8x8(half_rest(hi, w0, w1));
         }
     // ---- p.v: channels gr * DJ .. + DJ - 1 of keys 16 u + 2 c4 + {0, 1, 8, 9}
 #pragma unroll
@@ -461,12 +370,6 @@ __global__ void __launch_bounds__(kThreads)
   cp_async_wait_all();
   __syncwarp();
 
-  T* out = static_cast<T*>(p.out);
-  auto out_row = [&](int r) {
-    const int row = r0 + r;
-    return out + (static_cast<size_t>(b) * p.Sq + row / p.g) * p.ldo +
-           (static_cast<size_t>(hkv) * p.g + row % p.g) * DH;
-  };
   if constexpr (kSolo) {
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -476,7 +379,7 @@ __global__ void __launch_bounds__(kThreads)
         for (int x = 4; x <= 16; x <<= 1) l[n][z] += __shfl_xor_sync(0xffffffffu, l[n][z], x);
         const int r = 8 * n + 2 * c4 + z;
         if (r0 + r > last) continue;
-        const float down = l[n][z] == 0.0f ? 0.0f : pow2i(ew[n][z] - 15) / l[n][z];
+        const float down = l[n][z] == 0.0f ? 0.0f : 1.0f / l[n][z];
         constexpr int kPer = 16 / static_cast<int>(sizeof(T));
         Vec<T, kPer> v[DJ / kPer];
 #pragma unroll
@@ -484,30 +387,29 @@ __global__ void __launch_bounds__(kThreads)
           v[2 * j / kPer].v[2 * j % kPer] = from_f<T>(o[n][j][z] * down);
           v[(2 * j + 1) / kPer].v[(2 * j + 1) % kPer] = from_f<T>(o[n][j][2 + z] * down);
         }
-        T* dst = out_row(r) + gr * DJ;
+        T* dst = tile.out_row<T>(p, r0 + r, DH) + gr * DJ;
 #pragma unroll
         for (int j = 0; j < DJ / kPer; ++j) reinterpret_cast<Vec<T, kPer>*>(dst)[j] = v[j];
       }
     return;
   }
-  // ---- this warp's partial results: maximum, sum, and o in true scale, into its ring
+  // ---- this warp's partial results: reference, sum and o, into its ring
   float* s_o = reinterpret_cast<float*>(ring);  // [kRows][DH]
 #pragma unroll
   for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-      const float down = pow2i(ew[n][z] - 15);
 #pragma unroll
       for (int x = 4; x <= 16; x <<= 1) l[n][z] += __shfl_xor_sync(0xffffffffu, l[n][z], x);
       const int r = 8 * n + 2 * c4 + z;
       if (gr == 0) {
-        s_m[warp][r] = m[n][z];
+        s_m[warp][r] = ref[n][z];
         s_l[warp][r] = l[n][z];
       }
 #pragma unroll
       for (int j = 0; j < KS; j += 2)
         *reinterpret_cast<float4*>(s_o + r * DH + gr * DJ + 2 * j) =
-            make_float4(o[n][j][z] * down, o[n][j][2 + z] * down, o[n][j + 1][z] * down, o[n][j + 1][2 + z] * down);
+            make_float4(o[n][j][z], o[n][j][2 + z], o[n][j + 1][z], o[n][j + 1][2 + z]);
     }
   __syncthreads();
   // ---- the CTA's warps join, element by element (each read and written by one thread)
@@ -531,7 +433,7 @@ __global__ void __launch_bounds__(kThreads)
       s_cl[r] = ls;
     }
   }
-  auto store = [&](int r, int d, float v) { out_row(r)[d] = from_f<T>(v); };
+  auto store = [&](int r, int d, float v) { tile.out_row<T>(p, r0 + r, DH)[d] = from_f<T>(v); };
   const int n_rows = last - r0 + 1;  // rows of this tile that exist
   if (p.C == 1) {
     __syncthreads();
@@ -606,21 +508,8 @@ int launch(AttnKvParams p, cudaStream_t s) {
                               dim3(kThreads), C::kSmem, s, p));
     return DLM_OK;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.C));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.C;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  DLM_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_kv_kernel<T, DH, NR, false>, p));
+  DLM_CHECK_CUDA(launch_clusters(attn_kv_kernel<T, DH, NR, false>, static_cast<unsigned>(tiles * p.C), kThreads,
+                                 C::kSmem, p.C, s, p));
   return DLM_OK;
 }
 
@@ -628,7 +517,8 @@ template <typename T, int DH>
 int launch_rows(const AttnKvParams& p, cudaStream_t s) {
   const long long rows = static_cast<long long>(p.Sq) * p.g;
   if (rows <= 8) return launch<T, DH, 1>(p, s);
-  return launch<T, DH, 2>(p, s);
+  if (rows <= kAttnKvFewRows) return launch<T, DH, 2>(p, s);
+  return attn_kv_tc<T, DH>(p, s);
 }
 
 }  // namespace

@@ -1,0 +1,521 @@
+// Attention over the int8 K/V cache for many rows (prompt chunks), on tcgen05 (attention_kv.cu has
+// the formulas and the few-row kernel).
+//
+// One CTA takes 128 rows of one (sequence, kv head): row r is TMEM lane r.  Its key tiles (KT keys)
+// alternate between two streams A and B, each with its own scores and output accumulator, so that one
+// stream's products run under the other's softmax; a cluster of C CTAs may share a tile's keys.  All
+// partial results meet at the end in a fixed order (A with B in the CTA, then the CTAs).
+//   warps 0..3 / 4..7   softmax of stream A / B: thread = row; S from TMEM, weights w = p vscale
+//                       against the row's running reference, as fp16 pairs back into S's columns,
+//                       from where the second product takes its A operand;
+//   warps 8 / 9         MMA issuers of A / B: S = Q K^T (M 128, N KT, K DH), O += W V (M 128,
+//                       N DH, K KT, V as an MN-major operand);
+//   warps 10..13        the tiles' codes -> fp16 in the 128-byte-swizzled layout both products read,
+//                       with the tile's scales, through a ring of kStages tiles (the next tile's
+//                       codes are requested before the current one is converted).
+// The scales stay outside the products, as in the few-row kernel: codes are exact in fp16.  For fp32
+// inputs q and the weights are two fp16 terms each, and every product is issued for both.
+// Bound by the softmax's instruction issue (about ten instructions for two scores).
+#include "attention_kv.cuh"
+
+namespace dlm {
+
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kConvWarps = 4;
+constexpr int kTcThreads = (8 + 2 + kConvWarps) * 32;
+
+template <int DH, bool kSplit>
+struct TcCfg {
+  static constexpr int KT = kSplit ? 64 : 128;  // keys per tile
+  static constexpr int NT = kSplit ? 2 : 1;     // fp16 terms of q and of the weights
+  static constexpr int kHalves = DH / 64;       // 64-channel blocks (128-byte rows)
+  static constexpr int kQBytes = NT * kHalves * kRows * 128;
+  static constexpr int kTile = kHalves * KT * 128;  // K or V of a tile
+  static constexpr int kStages = kTile <= 8192 ? 4 : kTile <= 16384 ? 3 : 2;
+  static constexpr int kScales = 2 * KT * 4;  // kscale, vscale
+  static constexpr int kRing = kStages * 2 * kTile;
+  static constexpr int kOut = kRows * DH * 4;  // O of stream B, then the CTA's, over Q and the ring
+  static constexpr int kData = kQBytes + kRing > kOut ? kQBytes + kRing : kOut;
+  static constexpr int kSmem = kData + kStages * kScales + kRows * 5 * 4 + 256 + 1024;
+  // TMEM columns: S of A, S of B (the weights' first term in their first KT / 2), O of A, O of B, and
+  // the weights' second terms
+  static constexpr uint32_t kS = 0, kO = 2 * KT, kW2 = kO + 2 * DH;
+  static_assert(kW2 + (kSplit ? KT : 0) <= 512, "tensor memory");
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// 16 codes -> 16 fp16 values (two 16-byte pieces)
+__device__ __forceinline__ void expand16(uint4 c, uint4& a, uint4& b) {
+  const uint32_t x = c.x ^ 0x80808080u, y = c.y ^ 0x80808080u, z = c.z ^ 0x80808080u, w = c.w ^ 0x80808080u;
+  a = make_uint4(code_pair(x, 0x4140), code_pair(x, 0x4342), code_pair(y, 0x4140), code_pair(y, 0x4342));
+  b = make_uint4(code_pair(z, 0x4140), code_pair(z, 0x4342), code_pair(w, 0x4140), code_pair(w, 0x4342));
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attn_kv_tc_kernel(const AttnKvParams p) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  constexpr bool kScaled = !std::is_same<T, __half>::value;
+  using C = TcCfg<DH, kSplit>;
+  constexpr int KT = C::KT, NT = C::NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + C::kQBytes;
+  float* sScale = reinterpret_cast<float*>(smem + C::kData);  // [stage][2][KT]
+  float* s_qmul = sScale + C::kStages * 2 * KT;               // [kRows]
+  float* s_ref = s_qmul + kRows;                              // [2][kRows] of B, then of the CTA
+  float* s_l = s_ref + 2 * kRows;                             // [2][kRows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + 2 * kRows);
+  uint64_t* kv_full = bars;                  // [stages]
+  uint64_t* kv_empty = kv_full + C::kStages; // [stages]
+  uint64_t* s_full = kv_empty + C::kStages;  // [stream]
+  uint64_t* w_full = s_full + 2;             // [stream]
+  uint64_t* o_full = w_full + 2;             // [stream]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x % p.C);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&kv_full[s], kConvWarps * 32);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&w_full[s], kRows);
+      mbar_init(&o_full[s], 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  griddep_wait();  // inputs come from the previous kernel (programmatic dependent launch)
+  const AttnKvTile tile(p, static_cast<int>(blockIdx.x / p.C), kRows, threadIdx.x == 0);
+  const int n_tiles = (tile.n_keys + KT - 1) / KT;
+  // this CTA's tiles: rank + C * i, i = 0, 1, ..; tile i belongs to stream i & 1, stage i % kStages
+  const int n_mine = n_tiles > rank ? (n_tiles - rank + p.C - 1) / p.C : 0;
+
+  if (warp < 4) {
+    // ---- q as fp16 terms in shared memory (thread = row), rows beyond the last as zeros
+    const int row = threadIdx.x;
+    const bool in = tile.r0 + row <= tile.last;
+    const T* q = tile.q_row<T>(p, in ? tile.r0 + row : 0, DH);
+    constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+    float up = 1.0f, mul = p.scale_log2;
+    if constexpr (kScaled) {
+      float mx = 0.0f;
+      if (in)
+        for (int i = 0; i < DH / kPer; ++i) {
+          const Vec<T, kPer> v = reinterpret_cast<const Vec<T, kPer>*>(q)[i];
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, fabsf(to_f(v.v[j])));
+        }
+      const int e = q_up(mx);
+      up = pow2i(e);
+      mul *= pow2i(-e);
+    }
+    s_qmul[row] = mul;
+#pragma unroll
+    for (int i = 0; i < DH / 8; ++i) {
+      float f[8];
+#pragma unroll
+      for (int h = 0; h < 8 / kPer; ++h) {
+        Vec<T, kPer> v;
+        if (in) v = reinterpret_cast<const Vec<T, kPer>*>(q)[i * (8 / kPer) + h];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) f[h * kPer + j] = in ? to_f(v.v[j]) * up : 0.0f;
+      }
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        hi[j] = half_pair(f[2 * j], f[2 * j + 1]);
+        lo[j] = kSplit ? half_rest(hi[j], f[2 * j], f[2 * j + 1]) : 0u;
+      }
+      uint8_t* dst = sQ + (i / 8) * kRows * 128 + row * 128 + (((i % 8) ^ (row & 7)) << 4);
+      *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if constexpr (kSplit)
+        *reinterpret_cast<uint4*>(dst + C::kHalves * kRows * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = *tmem_slot;
+
+  float ref = kNoRef, l = 0.0f;  // of this thread's row (softmax warps)
+  if (warp >= 10) {
+    // ================================================================ codes -> fp16
+    const int t = threadIdx.x - 320;
+    constexpr int kPieces = DH / 16;                      // 16-code pieces of a row
+    constexpr int kEach = KT * kPieces / (kConvWarps * 32);  // pieces a thread converts, of K and of V
+    const size_t head = tile.head(p);
+    const int8_t* kb = p.kq + head * p.Lmax * DH;
+    const int8_t* vb = p.vq + head * p.Lmax * DH;
+    const float* ksb = p.ks + head * p.Lmax;
+    const float* vsb = p.vs + head * p.Lmax;
+    uint4 rk[kEach], rv[kEach];
+    float sk = 0.0f, sv = 0.0f;
+    auto request = [&](int i) {
+      const int k0 = (rank + p.C * i) * KT;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int id = e * kConvWarps * 32 + t;
+        const bool in = k0 + id / kPieces < tile.n_keys;
+        const size_t off = static_cast<size_t>(k0) * DH + static_cast<size_t>(id) * 16;
+        rk[e] = in ? __ldg(reinterpret_cast<const uint4*>(kb + off)) : make_uint4(0, 0, 0, 0);
+        rv[e] = in ? __ldg(reinterpret_cast<const uint4*>(vb + off)) : make_uint4(0, 0, 0, 0);
+      }
+      const bool in = t < KT && k0 + t < tile.n_keys;
+      sk = in ? __ldg(ksb + k0 + t) : 0.0f;
+      sv = in ? __ldg(vsb + k0 + t) : 0.0f;
+    };
+    if (n_mine > 0) request(0);
+    int st = 0;
+    uint32_t ph = 0;
+    for (int i = 0; i < n_mine; ++i) {
+      if (!mbar_wait(&kv_empty[st], ph ^ 1, abort_flag, p.status, kDevTimeoutProducer)) break;
+      uint8_t* dk = sKV + st * 2 * C::kTile;
+      uint8_t* dv = dk + C::kTile;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int id = e * kConvWarps * 32 + t;
+        const int r = id / kPieces, ch = id % kPieces;
+        // the second half's pieces go in the other order: no bank conflict with the first half's
+        const int odd = DH == 128 ? ch >> 2 : 0;
+        const int off = (ch >> 2) * KT * 128 + r * 128;
+        const int p0 = ((2 * (ch & 3) + odd) ^ (r & 7)) << 4, p1 = ((2 * (ch & 3) + 1 - odd) ^ (r & 7)) << 4;
+        uint4 a, b;
+        expand16(rk[e], a, b);
+        *reinterpret_cast<uint4*>(dk + off + p0) = odd ? b : a;
+        *reinterpret_cast<uint4*>(dk + off + p1) = odd ? a : b;
+        expand16(rv[e], a, b);
+        *reinterpret_cast<uint4*>(dv + off + p0) = odd ? b : a;
+        *reinterpret_cast<uint4*>(dv + off + p1) = odd ? a : b;
+      }
+      if (t < KT) {
+        sScale[st * 2 * KT + t] = sk;
+        sScale[st * 2 * KT + KT + t] = sv;
+      }
+      if (i + 1 < n_mine) request(i + 1);
+      fence_proxy_async_smem();
+      mbar_arrive(&kv_full[st]);
+      if (++st == C::kStages) {
+        st = 0;
+        ph ^= 1;
+      }
+    }
+  } else if (warp >= 8) {
+    // ================================================================ MMA issuer of one stream
+    if (lane == 0) {
+      const int sm = warp - 8;
+      constexpr uint32_t idesc_s = idesc_f16_f32(kRows, KT, false);
+      constexpr uint32_t idesc_o = idesc_f16_f32(kRows, DH, true);
+      const uint32_t ts = tbase + C::kS + sm * KT, to = tbase + C::kO + sm * DH;
+      for (int i = sm, n = 0; i < n_mine; i += 2, ++n) {
+        const int st = i % C::kStages;
+        if (!mbar_wait(&kv_full[st], (i / C::kStages) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        // the weights of the stream's previous tile lie in S's columns: its product has to be done
+        if (n > 0 && !mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        tc_fence_after();
+        const uint32_t k_addr = smem_u32(sKV + st * 2 * C::kTile), v_addr = k_addr + C::kTile;
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16_ss(ts, sw128_desc(smem_u32(sQ) + (x * C::kHalves + h) * kRows * 128 + k * 32, 16, 1024),
+                          sw128_desc(k_addr + h * KT * 128 + k * 32, 16, 1024), idesc_s,
+                          (x | h | k) != 0 ? 1u : 0u);
+        umma_commit(&s_full[sm]);
+        if (!mbar_wait(&w_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int k = 0; k < KT / 16; ++k)
+            umma_f16_ts(to, (x == 0 ? ts : tbase + C::kW2 + sm * (KT / 2)) + k * 8,
+                        sw128_desc(v_addr + k * 2048, KT * 128, 1024), idesc_o, (n | x | k) != 0 ? 1u : 0u);
+        umma_commit(&kv_empty[st]);
+        umma_commit(&o_full[sm]);
+      }
+      griddep_launch_dependents();
+    }
+  } else {
+    // ================================================================ softmax of one stream
+    const int sm = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tbase + lanes + C::kS + sm * KT, to = tbase + lanes + C::kO + sm * DH;
+    const uint32_t tw2 = tbase + lanes + C::kW2 + sm * (KT / 2);
+    const float qmul = s_qmul[row];
+    const int lim = tile.r0 + row <= tile.last ? tile.seen(p, tile.r0 + row) : tile.n_keys;
+    const uint64_t qmul2 = f2_pack(qmul, qmul);
+    int n = 0;
+    for (int i = sm; i < n_mine; i += 2, ++n) {
+      const float* sc = sScale + (i % C::kStages) * 2 * KT;
+      const int k0 = (rank + p.C * i) * KT;
+      const bool masked = k0 + KT > tile.n_all;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[sm], n & 1, abort_flag, p.status, kDevTimeoutSoftmax))) break;
+      tc_fence_after();
+      uint32_t w1[KT / 2], w2[kSplit ? KT / 2 : 1];
+      float big = 0.0f;
+      uint64_t sum = f2_pack(0.0f, 0.0f);
+      // weights of columns c .. c + 3 against `ref` (a masked key's scale may be anything)
+      auto weigh = [&](int c, const uint32_t* s, auto mask) {
+        const float4 ks = *reinterpret_cast<const float4*>(sc + c), vs = *reinterpret_cast<const float4*>(sc + KT + c);
+        const uint64_t nref = f2_pack(-ref, -ref);
+        const float k4[4] = {ks.x, ks.y, ks.z, ks.w}, v4[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const uint64_t kk = f2_fma(f2_pack(k4[j], k4[j + 1]), qmul2, f2_pack(0.0f, 0.0f));
+          float d0, d1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), kk, nref), d0, d1);
+          float e0 = fast_exp2(d0), e1 = fast_exp2(d1), x0 = e0 * v4[j], x1 = e1 * v4[j + 1];
+          if (mask) {
+            if (k0 + c + j >= lim) e0 = x0 = 0.0f;
+            if (k0 + c + j + 1 >= lim) e1 = x1 = 0.0f;
+          }
+          sum = f2_add(sum, f2_pack(e0, e1));
+          big = max3f(big, fabsf(x0), fabsf(x1));
+          w1[(c + j) / 2] = half_pair(x0, x1);
+          if constexpr (kSplit) w2[(c + j) / 2] = half_rest(w1[(c + j) / 2], x0, x1);
+        }
+      };
+      auto pass = [&](auto mask) {
+#pragma unroll
+        for (int c = 0; c < KT; c += 32) {
+          uint32_t s[32];
+          tmem_ld_32x32b_x32(ts + c, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) weigh(c + j, s + j, mask);
+        }
+      };
+      auto total = [&]() {
+        float a, b;
+        f2_unpack(sum, a, b);
+        return l + (a + b);
+      };
+      if (masked)
+        pass(std::true_type{});
+      else
+        pass(std::false_type{});
+      float lu = total();
+      if (__any_sync(0xffffffffu, big >= kMaxWeight || lu >= kMaxSum)) {
+        // the references move (the first tile, a score well above those so far, a large vscale)
+        float top = -INFINITY, top_w = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < KT; c += 16) {
+          uint32_t s[16];
+          tmem_ld_32x32b_x16(ts + c, s);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float x = k0 + c + j < lim ? __uint_as_float(s[j]) * (sc[c + j] * qmul) : -INFINITY;
+            top = fmaxf(top, x);
+            top_w = fmaxf(top_w, weight_log2(x, sc[KT + c + j]));
+          }
+        }
+        // this row's own need only: a row that fits keeps its reference and its weights
+        const float moved = big >= kMaxWeight || lu >= kMaxSum ? new_ref(ref, top, top_w) : ref;
+        const float alpha = fast_exp2(ref - moved);
+        ref = moved;
+        l *= alpha;
+        big = 0.0f;
+        sum = f2_pack(0.0f, 0.0f);
+        pass(std::true_type{});
+        lu = total();
+        if (n > 0) {  // O *= alpha (the stream's previous product is complete: S came after it)
+          const uint64_t a2 = f2_pack(alpha, alpha), z2 = f2_pack(0.0f, 0.0f);
+#pragma unroll 1
+          for (int c = 0; c < DH; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(to + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float x0, x1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), a2, z2), x0, x1);
+              r[j] = __float_as_uint(x0);
+              r[j + 1] = __float_as_uint(x1);
+            }
+            tmem_st_32x32b_x32(to + c, r);
+          }
+        }
+      }
+      l = lu;
+      // every S value is in registers: the weights take its first columns
+#pragma unroll
+      for (int c = 0; c < KT / 2; c += 32) {
+        tmem_st_32x32b_x32(ts + c, reinterpret_cast<const uint32_t(&)[32]>(w1[c]));
+        if constexpr (kSplit) tmem_st_32x32b_x32(tw2 + c, reinterpret_cast<const uint32_t(&)[32]>(w2[c]));
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&w_full[sm]);
+    }
+    if (n > 0) __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
+    tc_fence_after();
+  }
+  __syncthreads();  // every product is done: Q and the ring are free
+
+  // ---- stream B's result into shared memory, 16-byte pieces XORed with the row
+  float* s_out = reinterpret_cast<float*>(smem);
+  auto piece = [&](int row, int c) { return s_out + row * DH + ((c ^ (row & 7)) << 2); };
+  const bool two = n_mine > 1;
+  if (two && warp >= 4 && warp < 8) {
+    const int row = threadIdx.x & 127;
+    const uint32_t to = tbase + (static_cast<uint32_t>((warp & 3) * 32) << 16) + C::kO + DH;
+#pragma unroll 1
+    for (int c = 0; c < DH; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(to + c, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<uint4*>(piece(row, c / 4 + j)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+    }
+    s_ref[row] = ref;
+    s_l[row] = l;
+  }
+  __syncthreads();
+  // ---- A and B join (thread = row)
+  const bool alone = p.C == 1;
+  if (warp < 4) {
+    const int row = threadIdx.x;
+    const uint32_t to = tbase + (static_cast<uint32_t>(warp * 32) << 16) + C::kO;
+    float M = ref, fa = 1.0f, fb = 0.0f, L = l;
+    if (two) {
+      M = fmaxf(ref, s_ref[row]);
+      fa = fast_exp2(ref - M);
+      fb = fast_exp2(s_ref[row] - M);
+      L = fmaf(fa, l, fb * s_l[row]);
+    }
+    const bool in = tile.r0 + row <= tile.last;
+    T* dst = tile.out_row<T>(p, in ? tile.r0 + row : 0, DH);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll 1
+    for (int c = 0; c < DH; c += 32) {
+      float v[32];
+      uint32_t r[32];
+      if (n_mine > 0) {
+        tmem_ld_32x32b_x32(to + c, r);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = n_mine > 0 ? __uint_as_float(r[j]) : 0.0f;
+      if (two) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 o = *reinterpret_cast<const float4*>(piece(row, c / 4 + j));
+          const float w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int z = 0; z < 4; ++z) v[4 * j + z] = fmaf(fa, v[4 * j + z], fb * w[z]);
+        }
+      }
+      if (alone) {
+        if (in) {
+          constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+#pragma unroll
+          for (int j = 0; j < 32 / kPer; ++j) {
+            Vec<T, kPer> o;
+#pragma unroll
+            for (int z = 0; z < kPer; ++z) o.v[z] = from_f<T>(L == 0.0f ? 0.0f : v[j * kPer + z] * inv);
+            reinterpret_cast<Vec<T, kPer>*>(dst + c)[j] = o;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4*>(piece(row, c / 4 + j)) =
+              make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      }
+    }
+    if (!alone) {
+      s_ref[kRows + row] = M;
+      s_l[kRows + row] = L;
+    }
+  }
+  if (!alone) {
+    // ---- the cluster's CTAs join, each for its share of the tile
+    cluster_sync_all();
+    const int n_rows = tile.last - tile.r0 + 1;
+    for (int i = rank * kTcThreads + static_cast<int>(threadIdx.x); i < n_rows * DH; i += p.C * kTcThreads) {
+      const int row = i / DH, d = i % DH;
+      const uint32_t a_o = smem_u32(piece(row, d >> 2) + (d & 3));
+      const uint32_t a_m = smem_u32(&s_ref[kRows + row]), a_l = smem_u32(&s_l[kRows + row]);
+      float M = -INFINITY;
+      for (int c = 0; c < p.C; ++c) M = fmaxf(M, ld_dsmem(a_m, c));
+      float acc = 0.0f, L = 0.0f;
+      for (int c = 0; c < p.C; ++c) {
+        const float f = fast_exp2(ld_dsmem(a_m, c) - M);
+        acc = fmaf(f, ld_dsmem(a_o, c), acc);
+        L = fmaf(f, ld_dsmem(a_l, c), L);
+      }
+      tile.out_row<T>(p, tile.r0 + row, DH)[d] = from_f<T>(L == 0.0f ? 0.0f : acc / L);
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its shared memory
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) drain_sleep(200000);
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+}  // namespace
+
+template <typename T, int DH>
+int attn_kv_tc(const AttnKvParams& given, cudaStream_t s) {
+  using C = TcCfg<DH, sizeof(T) == 4>;
+  AttnKvParams p = given;
+  static bool done[64] = {false};
+  int dev = 0;
+  DLM_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !done[dev]) {
+    DLM_CHECK_CUDA(cudaFuncSetAttribute(attn_kv_tc_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        C::kSmem));
+    if (dev < 64) done[dev] = true;
+  }
+  const long long row_tiles = (static_cast<long long>(p.Sq) * p.g + kRows - 1) / kRows;
+  const long long tiles = row_tiles * p.B * p.Hkv;
+  DLM_REQUIRE(tiles < (1ll << 27), DLM_ERR_UNSUPPORTED, "attention_kv_i8: too many rows");
+  p.row_tiles = static_cast<int>(row_tiles);
+  p.tiles = static_cast<int>(tiles);
+  // CTAs per cluster: waves (one CTA per SM) times the longest row's keys, plus each CTA's fixed work
+  // (about as long as kFixed keys), is least
+  constexpr double kFixed = 512.0;
+  double best = 1e30;
+  for (int c = 1; c <= 8; ++c) {
+    const long long units = (p.Lmax + static_cast<long long>(C::KT) * c - 1) / (C::KT * c);
+    const double t = static_cast<double>((tiles * c + num_sms() - 1) / num_sms()) *
+                     (static_cast<double>(units * C::KT) + kFixed);
+    if (t < 0.97 * best) {
+      best = t;
+      p.C = c;
+    }
+  }
+  DLM_CHECK_CUDA(launch_clusters(attn_kv_tc_kernel<T, DH>, static_cast<unsigned>(tiles * p.C), kTcThreads, C::kSmem,
+                                 p.C, s, p));
+  return DLM_OK;
+}
+
+template int attn_kv_tc<float, 64>(const AttnKvParams&, cudaStream_t);
+template int attn_kv_tc<float, 128>(const AttnKvParams&, cudaStream_t);
+template int attn_kv_tc<__half, 64>(const AttnKvParams&, cudaStream_t);
+template int attn_kv_tc<__half, 128>(const AttnKvParams&, cudaStream_t);
+template int attn_kv_tc<__nv_bfloat16, 64>(const AttnKvParams&, cudaStream_t);
+template int attn_kv_tc<__nv_bfloat16, 128>(const AttnKvParams&, cudaStream_t);
+
+}  // namespace dlm

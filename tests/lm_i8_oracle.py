@@ -57,6 +57,7 @@ def attention(q, kq, ks, vq, vs, kv_len, q_len, causal, scale):
     mass = torch.zeros_like(out)                       # sum p |v|
     eps_s = torch.zeros(B, Sq, Hq, 1, dtype=torch.float64, device=q.device)
     terms = torch.zeros(B, 1, 1, 1, dtype=torch.float64, device=q.device)
+    floor = torch.zeros_like(eps_s)
     for b in range(B):
         n, m = min(max(int(kv_len[b]), 0), L), Sq if q_len is None else min(int(q_len[b]), Sq)
         terms[b] = n
@@ -71,6 +72,10 @@ def attention(q, kq, ks, vq, vs, kv_len, q_len, causal, scale):
                 p = torch.softmax(s, 0)
                 out[b, i, h] = p @ v
                 mass[b, i, h] = p @ v.abs()
+                # weights p vscale are held in fp16 terms scaled so that the row's largest is 2^14 or
+                # more: one below 2^-14 is off by half a subnormal step, 2^-25, which is 2^-39 of the
+                # largest, times a code of at most 127, for each of n keys
+                floor[b, i, h] = seen * 127 * 2.0 ** -39 * (p * vs[b, h // g, :seen].double().abs()).max()
                 big = (k.abs() @ q[b, i, h].double().abs()).max() * abs(scale)
                 # score error: Dh products summed in fp32 (each partial sum rounded or cut: 2^-23), q
                 # held to 2^-22, three fp32 factors and the subtraction of the maximum (2^-23 each of
@@ -79,5 +84,5 @@ def attention(q, kq, ks, vq, vs, kv_len, q_len, causal, scale):
     def bound(w_eps):
         # numerator and denominator both move by eps_s; sums over n keys: 16 at a time, then one
         # addition for every 16 keys and the joins of warps and blocks
-        return mass * (2 * eps_s + w_eps + (terms / 16 + 96) * 2.0 ** -23)
+        return mass * (2 * eps_s + w_eps + (terms / 16 + 96) * 2.0 ** -23) + floor
     return out, bound
