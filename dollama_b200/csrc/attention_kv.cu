@@ -24,8 +24,8 @@
 //
 // Precision: q is exact in fp16 for fp16, scaled per row by a power of two to [2^14, 2^15) for bf16
 // (exact down to 2^-25 of the row's maximum) and split into two fp16 terms for fp32.  The weights
-// w_ij = p_ij vscale_j are taken against a reference of their row's own that keeps the largest near
-// 2^14 (so a key that a row does not see has no part in it) and rounded to fp16 (a relative error of
+// w_ij = p_ij vscale_j are taken against a reference of their row's own that keeps them in fp16's
+// range (so a key that a row does not see has no part in it) and rounded to fp16 (a relative error of
 // 2^-11 each), for fp32 split into two terms.  Sums are fp32.
 #include "attention_kv.cuh"
 
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads)
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             top_w = fmaxf(top_w, __shfl_xor_sync(0xffffffffu, top_w, x));
           }
-          const float to = new_ref(ref[n][z], top, top_w);
+          const float to = new_ref<T>(ref[n][z], top, top_w);
           const float alpha = fast_exp2(ref[n][z] - to);
           ref[n][z] = to;
           lu[n][z] = l[n][z] * alpha;

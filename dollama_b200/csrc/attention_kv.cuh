@@ -80,14 +80,20 @@ struct AttnKvTile {
 };
 
 // The running reference of a row's weights: p_j = 2^(s_j - ref) and w_j = p_j vscale_j, with ref such
-// that the largest |w| when ref was set is 2^14 (fp16 keeps 11 bits of every weight down to 2^-28 of
-// it, and those below to 2^-39 of it) and p stays below 2^100; ref starts at kNoRef and moves only
-// when a weight would reach kMaxWeight or the sum kMaxSum.  Sum and products share the scale 2^-ref,
-// so out = o / l.
+// that the largest |w| when ref was set is 2^kTarget and p stays below 2^100; ref starts at kNoRef and
+// moves only when a weight would reach kMaxWeight or the sum kMaxSum.  Sum and products share the
+// scale 2^-ref, so out = o / l.  A lower target makes moves rarer (each costs a second pass over the
+// keys at hand: with 2^14 a tile of 128 keys x 32 rows moved one row or more most of the time, and
+// 2x500 queries over 4096 keys took 150 us) and costs range: fp16 keeps 11 bits of a weight down to
+// 2^-14, and an absolute 2^-25 below, which is 2^-35 of the largest weight for 16-bit types (2^-37 for
+// fp32, whose second terms reach 22 bits down to 2^-15 of it).
 constexpr float kNoRef = -1e30f, kMaxWeight = 60000.0f, kMaxSum = 0x1p122f;
+template <typename T>
+constexpr float kTarget = sizeof(T) == 4 ? 12.0f : 10.0f;
 // A new reference from the largest score and the largest score + log2 |vscale| (-inf for none).
+template <typename T>
 __device__ __forceinline__ float new_ref(float ref, float top, float top_w) {
-  return fmaxf(ref, fmaxf(top_w - 14.0f, top - 100.0f));
+  return fmaxf(ref, fmaxf(top_w - kTarget<T>, top - 100.0f));
 }
 // score + log2 |vscale|, -inf where vscale is zero or not finite
 __device__ __forceinline__ float weight_log2(float x, float vs) {

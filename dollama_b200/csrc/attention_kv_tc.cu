@@ -311,22 +311,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         pass(std::false_type{});
       float lu = total();
       if (__any_sync(0xffffffffu, big >= kMaxWeight || lu >= kMaxSum)) {
-        // the references move (the first tile, a score well above those so far, a large vscale)
-        float top = -INFINITY, top_w = -INFINITY;
+        // the references move, each by its own row's need only: a row that fits keeps its weights.  A
+        // finite overshoot says how far; the first tile (and scores or scales far beyond) ask for the
+        // maxima.
+        const bool need = big >= kMaxWeight || lu >= kMaxSum;
+        float moved = ref;
+        if (__any_sync(0xffffffffu, need && !(big < 1e30f && lu < kMaxSum))) {
+          float top = -INFINITY, top_w = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < KT; c += 16) {
-          uint32_t s[16];
-          tmem_ld_32x32b_x16(ts + c, s);
-          tmem_ld_wait();
+          for (int c = 0; c < KT; c += 32) {
+            uint32_t s[32];
+            tmem_ld_32x32b_x32(ts + c, s);
+            tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float x = k0 + c + j < lim ? __uint_as_float(s[j]) * (sc[c + j] * qmul) : -INFINITY;
-            top = fmaxf(top, x);
-            top_w = fmaxf(top_w, weight_log2(x, sc[KT + c + j]));
+            for (int j = 0; j < 32; ++j) {
+              const float x = k0 + c + j < lim ? __uint_as_float(s[j]) * (sc[c + j] * qmul) : -INFINITY;
+              top = fmaxf(top, x);
+              top_w = fmaxf(top_w, weight_log2(x, sc[KT + c + j]));
+            }
           }
+          if (need) moved = new_ref<T>(ref, top, top_w);
+        } else if (need) {
+          moved = ref + __log2f(big) - kTarget<T>;
         }
-        // this row's own need only: a row that fits keeps its reference and its weights
-        const float moved = big >= kMaxWeight || lu >= kMaxSum ? new_ref(ref, top, top_w) : ref;
         const float alpha = fast_exp2(ref - moved);
         ref = moved;
         l *= alpha;

@@ -72,10 +72,10 @@ def attention(q, kq, ks, vq, vs, kv_len, q_len, causal, scale):
                 p = torch.softmax(s, 0)
                 out[b, i, h] = p @ v
                 mass[b, i, h] = p @ v.abs()
-                # weights p vscale are held in fp16 terms scaled so that the row's largest is 2^14 or
-                # more: one below 2^-14 is off by half a subnormal step, 2^-25, which is 2^-39 of the
-                # largest, times a code of at most 127, for each of n keys
-                floor[b, i, h] = seen * 127 * 2.0 ** -39 * (p * vs[b, h // g, :seen].double().abs()).max()
+                # weights p vscale are held in fp16 terms scaled so that the row's largest is 2^10 or
+                # more: one below 2^-14 is off by half a subnormal step, 2^-25, which is 2^-35 of the
+                # largest (fp32: 2^12, 2^-37), times a code of at most 127, for each of n keys
+                floor[b, i, h] = seen * 127 * 2.0 ** (-37 if q.dtype == torch.float32 else -35) * (p * vs[b, h // g, :seen].double().abs()).max()
                 big = (k.abs() @ q[b, i, h].double().abs()).max() * abs(scale)
                 # score error: Dh products summed in fp32 (each partial sum rounded or cut: 2^-23), q
                 # held to 2^-22, three fp32 factors and the subtraction of the maximum (2^-23 each of
