@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int st = 0;
     uint32_t ph = 0;
     for (int i = 0; i < n_mine; ++i) {
-      if (!mbar_wait_spin(&kv_empty[st], ph ^ 1, abort_flag, p.status, kDevTimeoutProducer)) break;
+      if (!mbar_wait(&kv_empty[st], ph ^ 1, abort_flag, p.status, kDevTimeoutProducer)) break;
       uint8_t* dk = sKV + st * 2 * C::kTile;
       uint8_t* dv = dk + C::kTile;
 #pragma unroll
@@ -222,9 +222,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t ts = tbase + C::kS + sm * KT, to = tbase + C::kO + sm * DH;
       for (int i = sm, n = 0; i < n_mine; i += 2, ++n) {
         const int st = i % C::kStages;
-        if (!mbar_wait_spin(&kv_full[st], (i / C::kStages) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        if (!mbar_wait(&kv_full[st], (i / C::kStages) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
         // the weights of the stream's previous tile lie in S's columns: its product has to be done
-        if (n > 0 && !mbar_wait_spin(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        if (n > 0 && !mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
         tc_fence_after();
         const uint32_t k_addr = smem_u32(sKV + st * 2 * C::kTile), v_addr = k_addr + C::kTile;
 #pragma unroll
@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                           sw128_desc(k_addr + h * KT * 128 + k * 32, 16, 1024), idesc_s,
                           (x | h | k) != 0 ? 1u : 0u);
         umma_commit(&s_full[sm]);
-        if (!mbar_wait_spin(&w_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        if (!mbar_wait(&w_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma)) break;
         tc_fence_after();
 #pragma unroll
         for (int x = 0; x < NT; ++x)
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float* sc = sScale + (i % C::kStages) * 2 * KT;
       const int k0 = (rank + p.C * i) * KT;
       const bool masked = k0 + KT > tile.n_all;
-      if (!__all_sync(0xffffffffu, mbar_wait_spin(&s_full[sm], n & 1, abort_flag, p.status, kDevTimeoutSoftmax))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[sm], n & 1, abort_flag, p.status, kDevTimeoutSoftmax))) break;
       tc_fence_after();
       uint32_t w1[KT / 2], w2[kSplit ? KT / 2 : 1];
       float big = 0.0f;
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_before();
       mbar_arrive(&w_full[sm]);
     }
-    if (n > 0) __all_sync(0xffffffffu, mbar_wait_spin(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
+    if (n > 0) __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
     tc_fence_after();
   }
   __syncthreads();  // every product is done: Q and the ring are free

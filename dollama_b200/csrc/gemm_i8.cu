@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tile_at(p, t, mt, nt);
         const int a0 = (kPair ? 2 * mt + rank : mt) * kBM, b0 = (kPair ? 2 * nt + rank : nt) * 128;
         for (int kb = 0; kb < nkb; kb += C::kSub) {
-          ok = mbar_wait_spin(&empty[st], ph ^ 1, abort_flag, p.status, kDevTimeoutProducer);
+          ok = mbar_wait(&empty[st], ph ^ 1, abort_flag, p.status, kDevTimeoutProducer);
           if (!ok) break;
           const int nsub = min(C::kSub, nkb - kb);
           // a pair's copies, both CTAs', complete on the even CTA's barrier
@@ -254,11 +254,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int t = first; t < tiles && ok; t += step, ++i) {
         const int acc = i & 1;
-        ok = mbar_wait_spin(&tempty[acc], ((i >> 1) & 1) ^ 1, abort_flag, p.status, kDevTimeoutMma);
+        ok = mbar_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, abort_flag, p.status, kDevTimeoutMma);
         tc_fence_after();
         const uint32_t d = tbase + static_cast<uint32_t>(acc * C::kBN);
         for (int kb = 0; kb < nkb && ok; kb += C::kSub) {
-          ok = mbar_wait_spin(&full[st], ph, abort_flag, p.status, kDevTimeoutMma);
+          ok = mbar_wait(&full[st], ph, abort_flag, p.status, kDevTimeoutMma);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int mt, nt;
       tile_at(p, t, mt, nt);
       const int acc = i & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait_spin(&tfull[acc], (i >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue)))
+      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (i >> 1) & 1, abort_flag, p.status, kDevTimeoutEpilogue)))
         break;
       tc_fence_after();
       const uint32_t ta = tbase + (static_cast<uint32_t>(quad * 32) << 16) +
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(kKThreads)
       int st = 0;
       uint32_t ph = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_spin(&empty[st], ph ^ 1, abort_flag, p.status, kDevTimeoutProducer)) break;
+        if (!mbar_wait(&empty[st], ph ^ 1, abort_flag, p.status, kDevTimeoutProducer)) break;
         mbar_arrive_expect_tx(&full[st], kSubBytes + C::kStageB);
         tma_load_2d(sA + st * kSubBytes, &tmW, &full[st], kb * kKB, n0);
         tma_load_2d(sB + st * C::kStageB, &tmX, &full[st], kb * kKB, m0);
@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kKThreads)
       uint32_t ph = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1 && ok; ++kb) {
-        ok = mbar_wait_spin(&full[st], ph, abort_flag, p.status, kDevTimeoutMma);
+        ok = mbar_wait(&full[st], ph, abort_flag, p.status, kDevTimeoutMma);
         if (!ok) break;
         tc_fence_after();
         const uint32_t a = smem_u32(sA + st * kSubBytes), b = smem_u32(sB + st * C::kStageB);
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kKThreads)
   } else {
     // partial sums [token][channel] into the ring, which the last MMA has left
     const int quad = warp & 3;
-    if (__all_sync(0xffffffffu, mbar_wait_spin(acc_full, 0, abort_flag, p.status, kDevTimeoutEpilogue))) {
+    if (__all_sync(0xffffffffu, mbar_wait(acc_full, 0, abort_flag, p.status, kDevTimeoutEpilogue))) {
       tc_fence_after();
       const uint32_t ta = tbase + (static_cast<uint32_t>(quad * 32) << 16);
       int* part = reinterpret_cast<int*>(smem) + quad * 32 + lane;

@@ -98,26 +98,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-// mbar_wait for short hand-overs: the clock, whose first reading would delay the wake-up of a wait that
-// is over in a microsecond, is asked only after kSpinPolls polls, and every kSpinPolls from then on.
-constexpr uint32_t kSpinPolls = 512;
-__device__ __forceinline__ bool mbar_wait_spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                               int* status, int code) {
-  unsigned long long t0 = 0;
-  for (uint32_t it = 1; !mbar_try_wait(bar, parity); ++it) {
-    if (it % kSpinPolls != 0) continue;
-    if (*abort_flag) return false;
-    const unsigned long long now = globaltimer_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitTimeoutNs) {
-      if (status) atomicCAS(status, 0, code);
-      *abort_flag = 1;
-      return false;
-    }
-  }
-  return true;
-}
-
 // Waits (bounded) until the global flag holds `want`, with acquire semantics: every write the
 // signalling thread made before its release store is visible afterwards.
 __device__ __forceinline__ bool flag_wait_acquire(const int* flag, int want, volatile int* abort_flag,
