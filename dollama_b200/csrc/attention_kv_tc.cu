@@ -2,20 +2,24 @@
 // the formulas and the few-row kernel).
 //
 // One CTA takes 128 rows of one (sequence, kv head): row r is TMEM lane r.  Its key tiles (KT keys)
-// alternate between two streams A and B, each with its own scores and output accumulator, so that one
-// stream's products run under the other's softmax; a cluster of C CTAs may share a tile's keys.  All
-// partial results meet at the end in a fixed order (A with B in the CTA, then the CTAs).
-//   warps 0..3 / 4..7   softmax of stream A / B: thread = row; S from TMEM, weights w = p vscale
-//                       against the row's running reference, as fp16 pairs back into S's columns,
-//                       from where the second product takes its A operand;
+// alternate between two streams A and B, each with its own scores, weights and output accumulator, so
+// that one stream's products run under the other's softmax; a cluster of C CTAs may share a tile's
+// keys.  All partial results meet at the end in a fixed order (A with B in the CTA, then the CTAs).
+//   warps 0..3 / 4..7   softmax of stream A / B: thread = row; S from TMEM (32 columns at a time, the
+//                       next ones requested before the current ones are exponentiated), weights
+//                       w = p vscale against the row's running reference, as fp16 pairs into the
+//                       stream's W columns, from where the second product takes its A operand;
 //   warps 8 / 9         MMA issuers of A / B: S = Q K^T (M 128, N KT, K DH), O += W V (M 128,
-//                       N DH, K KT, V as an MN-major operand);
+//                       N DH, K KT, V as an MN-major operand); the stream's next S is issued as soon
+//                       as the softmax is done with the last one, before W V;
 //   warps 10..13        the tiles' codes -> fp16 in the 128-byte-swizzled layout both products read,
 //                       with the tile's scales, through a ring of kStages tiles (the next tile's
 //                       codes are requested before the current one is converted).
-// The scales stay outside the products, as in the few-row kernel: codes are exact in fp16.  For fp32
-// inputs q and the weights are two fp16 terms each, and every product is issued for both.
-// Bound by the softmax's instruction issue (about ten instructions for two scores).
+// The scales stay outside the products, as in the few-row kernel: codes are exact in fp16.  q is
+// scaled by one power of two for the tile's rows (16-bit values keep all their bits down to 2^-29 of
+// the tile's largest; what is lost below moves no score by 2^-38 of the largest one), which the staged
+// kscale takes back.  For fp32 inputs q and the weights are two fp16 terms each, and every product is
+// issued for both.  Bound by the softmax's instruction issue.
 #include "attention_kv.cuh"
 
 namespace dlm {
@@ -28,21 +32,20 @@ constexpr int kTcThreads = (8 + 2 + kConvWarps) * 32;
 
 template <int DH, bool kSplit>
 struct TcCfg {
-  static constexpr int KT = kSplit ? 64 : 128;  // keys per tile
-  static constexpr int NT = kSplit ? 2 : 1;     // fp16 terms of q and of the weights
-  static constexpr int kHalves = DH / 64;       // 64-channel blocks (128-byte rows)
+  static constexpr int KT = kSplit || DH == 128 ? 64 : 128;  // keys per tile
+  static constexpr int NT = kSplit ? 2 : 1;                  // fp16 terms of q and of the weights
+  static constexpr int kHalves = DH / 64;                    // 64-channel blocks (128-byte rows)
   static constexpr int kQBytes = NT * kHalves * kRows * 128;
   static constexpr int kTile = kHalves * KT * 128;  // K or V of a tile
-  static constexpr int kStages = kTile <= 8192 ? 4 : kTile <= 16384 ? 3 : 2;
+  static constexpr int kStages = kTile <= 8192 ? 4 : 3;
   static constexpr int kScales = 2 * KT * 4;  // kscale, vscale
   static constexpr int kRing = kStages * 2 * kTile;
   static constexpr int kOut = kRows * DH * 4;  // O of stream B, then the CTA's, over Q and the ring
   static constexpr int kData = kQBytes + kRing > kOut ? kQBytes + kRing : kOut;
-  static constexpr int kSmem = kData + kStages * kScales + kRows * 5 * 4 + 256 + 1024;
-  // TMEM columns: S of A, S of B (the weights' first term in their first KT / 2), O of A, O of B, and
-  // the weights' second terms
-  static constexpr uint32_t kS = 0, kO = 2 * KT, kW2 = kO + 2 * DH;
-  static_assert(kW2 + (kSplit ? KT : 0) <= 512, "tensor memory");
+  static constexpr int kSmem = kData + kStages * kScales + kRows * 4 * 4 + 512 + 1024;
+  // TMEM columns: S, O and W of the two streams
+  static constexpr uint32_t kS = 0, kO = 2 * KT, kW = kO + 2 * DH, kWCols = NT * KT / 2;
+  static_assert(kW + 2 * kWCols <= 512, "tensor memory");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -66,8 +69,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + C::kQBytes;
   float* sScale = reinterpret_cast<float*>(smem + C::kData);  // [stage][2][KT]
-  float* s_qmul = sScale + C::kStages * 2 * KT;               // [kRows]
-  float* s_ref = s_qmul + kRows;                              // [2][kRows] of B, then of the CTA
+  float* s_ref = sScale + C::kStages * 2 * KT;                // [2][kRows] of B, then of the CTA
   float* s_l = s_ref + 2 * kRows;                             // [2][kRows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + 2 * kRows);
   uint64_t* kv_full = bars;                  // [stages]
@@ -77,6 +79,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* o_full = w_full + 2;             // [stream]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* s_top = reinterpret_cast<float*>(tmem_slot + 2);  // [4] largest |q| of the four warps' rows
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x % p.C);
@@ -103,35 +106,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // this CTA's tiles: rank + C * i, i = 0, 1, ..; tile i belongs to stream i & 1, stage i % kStages
   const int n_mine = n_tiles > rank ? (n_tiles - rank + p.C - 1) / p.C : 0;
 
-  if (warp < 4) {
-    // ---- q as fp16 terms in shared memory (thread = row), rows beyond the last as zeros
-    const int row = threadIdx.x;
-    const bool in = tile.r0 + row <= tile.last;
-    const T* q = tile.q_row<T>(p, in ? tile.r0 + row : 0, DH);
-    constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-    float up = 1.0f, mul = p.scale_log2;
-    if constexpr (kScaled) {
-      float mx = 0.0f;
-      if (in)
-        for (int i = 0; i < DH / kPer; ++i) {
-          const Vec<T, kPer> v = reinterpret_cast<const Vec<T, kPer>*>(q)[i];
+  // ---- q as fp16 terms in shared memory (thread = row), rows beyond the last as zeros
+  const bool q_in = warp < 4 && tile.r0 + static_cast<int>(threadIdx.x) <= tile.last;
+  const T* q = tile.q_row<T>(p, q_in ? tile.r0 + static_cast<int>(threadIdx.x) : 0, DH);
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+  float up = 1.0f, qmul = p.scale_log2;
+  if constexpr (kScaled) {
+    float mx = 0.0f;
+    if (q_in)
+      for (int i = 0; i < DH / kPer; ++i) {
+        const Vec<T, kPer> v = reinterpret_cast<const Vec<T, kPer>*>(q)[i];
 #pragma unroll
-          for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, fabsf(to_f(v.v[j])));
-        }
-      const int e = q_up(mx);
-      up = pow2i(e);
-      mul *= pow2i(-e);
-    }
-    s_qmul[row] = mul;
+        for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, fabsf(to_f(v.v[j])));
+      }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0 && warp < 4) s_top[warp] = mx;
+    __syncthreads();
+    const int e = q_up(fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3])));
+    up = pow2i(e);
+    qmul *= pow2i(-e);
+  }
+  if (warp < 4) {
+    const int row = threadIdx.x;
 #pragma unroll
     for (int i = 0; i < DH / 8; ++i) {
       float f[8];
 #pragma unroll
       for (int h = 0; h < 8 / kPer; ++h) {
         Vec<T, kPer> v;
-        if (in) v = reinterpret_cast<const Vec<T, kPer>*>(q)[i * (8 / kPer) + h];
+        if (q_in) v = reinterpret_cast<const Vec<T, kPer>*>(q)[i * (8 / kPer) + h];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) f[h * kPer + j] = in ? to_f(v.v[j]) * up : 0.0f;
+        for (int j = 0; j < kPer; ++j) f[h * kPer + j] = q_in ? to_f(v.v[j]) * up : 0.0f;
       }
       uint32_t hi[4], lo[4];
 #pragma unroll
@@ -202,7 +208,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         *reinterpret_cast<uint4*>(dv + off + p1) = odd ? a : b;
       }
       if (t < KT) {
-        sScale[st * 2 * KT + t] = sk;
+        sScale[st * 2 * KT + t] = sk * qmul;
         sScale[st * 2 * KT + KT + t] = sv;
       }
       if (i + 1 < n_mine) request(i + 1);
@@ -220,13 +226,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       constexpr uint32_t idesc_s = idesc_f16_f32(kRows, KT, false);
       constexpr uint32_t idesc_o = idesc_f16_f32(kRows, DH, true);
       const uint32_t ts = tbase + C::kS + sm * KT, to = tbase + C::kO + sm * DH;
-      for (int i = sm, n = 0; i < n_mine; i += 2, ++n) {
+      const uint32_t tw = tbase + C::kW + sm * C::kWCols;
+      // S of the CTA's tile i, once its codes are there
+      auto scores = [&](int i) -> bool {
         const int st = i % C::kStages;
-        if (!mbar_wait(&kv_full[st], (i / C::kStages) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
-        // the weights of the stream's previous tile lie in S's columns: its product has to be done
-        if (n > 0 && !mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        if (!mbar_wait(&kv_full[st], (i / C::kStages) & 1, abort_flag, p.status, kDevTimeoutMma)) return false;
         tc_fence_after();
-        const uint32_t k_addr = smem_u32(sKV + st * 2 * C::kTile), v_addr = k_addr + C::kTile;
+        const uint32_t k_addr = smem_u32(sKV + st * 2 * C::kTile);
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -237,14 +243,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                           sw128_desc(k_addr + h * KT * 128 + k * 32, 16, 1024), idesc_s,
                           (x | h | k) != 0 ? 1u : 0u);
         umma_commit(&s_full[sm]);
-        if (!mbar_wait(&w_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma)) break;
+        return true;
+      };
+      bool ok = sm >= n_mine || scores(sm);
+      for (int i = sm, n = 0; ok && i < n_mine; i += 2, ++n) {
+        const int st = i % C::kStages;
+        ok = mbar_wait(&w_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma);
+        if (ok && i + 2 < n_mine) ok = scores(i + 2);  // the softmax is done with S
+        if (!ok) break;
         tc_fence_after();
+        const uint32_t v_addr = smem_u32(sKV + st * 2 * C::kTile) + C::kTile;
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
           for (int k = 0; k < KT / 16; ++k)
-            umma_f16_ts(to, (x == 0 ? ts : tbase + C::kW2 + sm * (KT / 2)) + k * 8,
-                        sw128_desc(v_addr + k * 2048, KT * 128, 1024), idesc_o, (n | x | k) != 0 ? 1u : 0u);
+            umma_f16_ts(to, tw + x * (KT / 2) + k * 8, sw128_desc(v_addr + k * 2048, KT * 128, 1024), idesc_o,
+                        (n | x | k) != 0 ? 1u : 0u);
         umma_commit(&kv_empty[st]);
         umma_commit(&o_full[sm]);
       }
@@ -255,68 +269,89 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int sm = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tbase + lanes + C::kS + sm * KT, to = tbase + lanes + C::kO + sm * DH;
-    const uint32_t tw2 = tbase + lanes + C::kW2 + sm * (KT / 2);
-    const float qmul = s_qmul[row];
+    const uint32_t tw = tbase + lanes + C::kW + sm * C::kWCols;
     const int lim = tile.r0 + row <= tile.last ? tile.seen(p, tile.r0 + row) : tile.n_keys;
-    const uint64_t qmul2 = f2_pack(qmul, qmul);
     int n = 0;
-    for (int i = sm; i < n_mine; i += 2, ++n) {
+    bool ok = true;
+    for (int i = sm; i < n_mine && ok; i += 2, ++n) {
       const float* sc = sScale + (i % C::kStages) * 2 * KT;
       const int k0 = (rank + p.C * i) * KT;
       const bool masked = k0 + KT > tile.n_all;
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[sm], n & 1, abort_flag, p.status, kDevTimeoutSoftmax))) break;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sm], n & 1, abort_flag, p.status, kDevTimeoutSoftmax));
+      if (!ok) break;
       tc_fence_after();
-      uint32_t w1[KT / 2], w2[kSplit ? KT / 2 : 1];
-      float big = 0.0f;
-      uint64_t sum = f2_pack(0.0f, 0.0f);
-      // weights of columns c .. c + 3 against `ref` (a masked key's scale may be anything)
-      auto weigh = [&](int c, const uint32_t* s, auto mask) {
-        const float4 ks = *reinterpret_cast<const float4*>(sc + c), vs = *reinterpret_cast<const float4*>(sc + KT + c);
+      bool w_free = n == 0;  // the stream's previous product has read W
+      for (int tries = 0;; ++tries) {
+        float big = 0.0f;
+        uint64_t sum = f2_pack(0.0f, 0.0f);
         const uint64_t nref = f2_pack(-ref, -ref);
-        const float k4[4] = {ks.x, ks.y, ks.z, ks.w}, v4[4] = {vs.x, vs.y, vs.z, vs.w};
+        // weights of columns c .. c + 31 against `ref` (a masked key's scale may be anything)
+        auto weigh = [&](int c, const uint32_t (&s)[32], auto mask) {
+          uint32_t w1[16], w2[kSplit ? 16 : 1];
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          const uint64_t kk = f2_fma(f2_pack(k4[j], k4[j + 1]), qmul2, f2_pack(0.0f, 0.0f));
-          float d0, d1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), kk, nref), d0, d1);
-          float e0 = fast_exp2(d0), e1 = fast_exp2(d1), x0 = e0 * v4[j], x1 = e1 * v4[j + 1];
-          if (mask) {
-            if (k0 + c + j >= lim) e0 = x0 = 0.0f;
-            if (k0 + c + j + 1 >= lim) e1 = x1 = 0.0f;
+          for (int j = 0; j < 32; j += 4) {
+            const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(sc + c + j);
+            const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(sc + KT + c + j);
+#pragma unroll
+            for (int z = 0; z < 4; z += 2) {
+              float d0, d1, x0, x1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(s[j + z]), __uint_as_float(s[j + z + 1])), z ? ks.y : ks.x, nref),
+                        d0, d1);
+              float e0 = fast_exp2(d0), e1 = fast_exp2(d1);
+              const uint64_t e = f2_pack(e0, e1);
+              f2_unpack(f2_mul(e, z ? vs.y : vs.x), x0, x1);
+              if (mask) {
+                if (k0 + c + j + z >= lim) e0 = x0 = 0.0f;
+                if (k0 + c + j + z + 1 >= lim) e1 = x1 = 0.0f;
+                sum = f2_add(sum, f2_pack(e0, e1));
+              } else {
+                sum = f2_add(sum, e);
+              }
+              big = max3f(big, fabsf(x0), fabsf(x1));
+              w1[(j + z) / 2] = half_pair(x0, x1);
+              if constexpr (kSplit) w2[(j + z) / 2] = half_rest(w1[(j + z) / 2], x0, x1);
+            }
           }
-          sum = f2_add(sum, f2_pack(e0, e1));
-          big = max3f(big, fabsf(x0), fabsf(x1));
-          w1[(c + j) / 2] = half_pair(x0, x1);
-          if constexpr (kSplit) w2[(c + j) / 2] = half_rest(w1[(c + j) / 2], x0, x1);
-        }
-      };
-      auto pass = [&](auto mask) {
-#pragma unroll
-        for (int c = 0; c < KT; c += 32) {
-          uint32_t s[32];
-          tmem_ld_32x32b_x32(ts + c, s);
+          if (!w_free) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
+            tc_fence_after();
+            w_free = true;
+          }
+          tmem_st_32x32b_x16(tw + c / 2, w1);
+          if constexpr (kSplit) tmem_st_32x32b_x16(tw + KT / 2 + c / 2, w2);
+        };
+        auto pass = [&](auto mask) {
+          uint32_t s0[32], s1[32];
+          tmem_ld_32x32b_x32(ts, s0);
           tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) weigh(c + j, s + j, mask);
-        }
-      };
-      auto total = [&]() {
+#pragma unroll 1
+          for (int c = 0; c < KT; c += 64) {
+            tmem_ld_32x32b_x32(ts + c + 32, s1);
+            weigh(c, s0, mask);
+            tmem_ld_wait();
+            if (c + 64 < KT) tmem_ld_32x32b_x32(ts + c + 64, s0);
+            weigh(c + 32, s1, mask);
+            tmem_ld_wait();
+          }
+        };
+        if (masked)
+          pass(std::true_type{});
+        else
+          pass(std::false_type{});
         float a, b;
         f2_unpack(sum, a, b);
-        return l + (a + b);
-      };
-      if (masked)
-        pass(std::true_type{});
-      else
-        pass(std::false_type{});
-      float lu = total();
-      if (__any_sync(0xffffffffu, big >= kMaxWeight || lu >= kMaxSum)) {
-        // the references move, each by its own row's need only: a row that fits keeps its weights.  A
-        // finite overshoot says how far; the first tile (and scores or scales far beyond) ask for the
-        // maxima.
+        const float lu = l + (a + b);
         const bool need = big >= kMaxWeight || lu >= kMaxSum;
+        if (!ok || tries == 2 || !__any_sync(0xffffffffu, need)) {
+          l = lu;
+          break;
+        }
+        // the references move, each by its own row's need only (a row that fits keeps its weights),
+        // and the pass is repeated, twice at most (infinite scores or scales never fit).  A finite
+        // overshoot says how far; the first tile, scores or scales far beyond, and a second try ask for
+        // the maxima.
         float moved = ref;
-        if (__any_sync(0xffffffffu, need && !(big < 1e30f && lu < kMaxSum))) {
+        if (__any_sync(0xffffffffu, need && !(tries == 0 && big < 1e30f && lu < kMaxSum))) {
           float top = -INFINITY, top_w = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < KT; c += 32) {
@@ -325,7 +360,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-              const float x = k0 + c + j < lim ? __uint_as_float(s[j]) * (sc[c + j] * qmul) : -INFINITY;
+              const float x = k0 + c + j < lim ? __uint_as_float(s[j]) * sc[c + j] : -INFINITY;
               top = fmaxf(top, x);
               top_w = fmaxf(top_w, weight_log2(x, sc[KT + c + j]));
             }
@@ -337,12 +372,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float alpha = fast_exp2(ref - moved);
         ref = moved;
         l *= alpha;
-        big = 0.0f;
-        sum = f2_pack(0.0f, 0.0f);
-        pass(std::true_type{});
-        lu = total();
-        if (n > 0) {  // O *= alpha (the stream's previous product is complete: S came after it)
-          const uint64_t a2 = f2_pack(alpha, alpha), z2 = f2_pack(0.0f, 0.0f);
+        if (n > 0) {  // O *= alpha (the stream's previous product is complete)
+          const uint64_t a2 = f2_pack(alpha, alpha);
 #pragma unroll 1
           for (int c = 0; c < DH; c += 32) {
             uint32_t r[32];
@@ -351,7 +382,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               float x0, x1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), a2, z2), x0, x1);
+              f2_unpack(f2_mul(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), a2), x0, x1);
               r[j] = __float_as_uint(x0);
               r[j + 1] = __float_as_uint(x1);
             }
@@ -359,18 +390,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
-      l = lu;
-      // every S value is in registers: the weights take its first columns
-#pragma unroll
-      for (int c = 0; c < KT / 2; c += 32) {
-        tmem_st_32x32b_x32(ts + c, reinterpret_cast<const uint32_t(&)[32]>(w1[c]));
-        if constexpr (kSplit) tmem_st_32x32b_x32(tw2 + c, reinterpret_cast<const uint32_t(&)[32]>(w2[c]));
-      }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&w_full[sm]);
     }
-    if (n > 0) __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
+    if (ok && n > 0)
+      __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
     tc_fence_after();
   }
   __syncthreads();  // every product is done: Q and the ring are free
@@ -431,7 +456,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       if (alone) {
         if (in) {
-          constexpr int kPer = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
           for (int j = 0; j < 32 / kPer; ++j) {
             Vec<T, kPer> o;
