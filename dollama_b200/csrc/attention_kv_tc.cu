@@ -5,10 +5,12 @@
 // alternate between two streams A and B, each with its own scores, weights and output accumulator, so
 // that one stream's products run under the other's softmax; a cluster of C CTAs may share a tile's
 // keys.  All partial results meet at the end in a fixed order (A with B in the CTA, then the CTAs).
-//   warps 0..3 / 4..7   softmax of stream A / B: thread = row; S from TMEM (32 columns at a time, the
-//                       next ones requested before the current ones are exponentiated), weights
-//                       w = p vscale against the row's running reference, as fp16 pairs into the
-//                       stream's W columns, from where the second product takes its A operand;
+//   warps 0..3 / 4..7   softmax of stream A / B: S from TMEM (32 columns at a time, the next ones
+//                       requested before the current ones are exponentiated), weights w = p vscale
+//                       against each row's running reference, as fp16 pairs into the stream's W
+//                       columns, from where the second product takes its A operand.  A lane takes
+//                       two of eight columns of four rows (the 16x256b pieces), so that a key's
+//                       scales, read from shared memory, serve four scores;
 //   warps 8 / 9         MMA issuers of A / B: S = Q K^T (M 128, N KT, K DH), O += W V (M 128,
 //                       N DH, K KT, V as an MN-major operand); the stream's next S is issued as soon
 //                       as the softmax is done with the last one, before W V;
@@ -69,7 +71,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + C::kQBytes;
   float* sScale = reinterpret_cast<float*>(smem + C::kData);  // [stage][2][KT]
-  float* s_ref = sScale + C::kStages * 2 * KT;                // [2][kRows] of B, then of the CTA
+  float* s_ref = sScale + C::kStages * 2 * KT;                // [2][kRows] of A and B, then of the CTA
   float* s_l = s_ref + 2 * kRows;                             // [2][kRows]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + 2 * kRows);
   uint64_t* kv_full = bars;                  // [stages]
@@ -157,7 +159,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
 
-  float ref = kNoRef, l = 0.0f;  // of this thread's row (softmax warps)
   if (warp >= 10) {
     // ================================================================ codes -> fp16
     const int t = threadIdx.x - 320;
@@ -266,50 +267,62 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else {
     // ================================================================ softmax of one stream
-    const int sm = warp >> 2, row = threadIdx.x & 127;
+    const int sm = warp >> 2, gr = lane >> 2, c4 = lane & 3;
+    const int row0 = (warp & 3) * 32 + gr;  // this lane's rows: row0 + 8 y
+    constexpr uint32_t kHalf = 16u << 16;   // TMEM address of 16 lanes further
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tbase + lanes + C::kS + sm * KT, to = tbase + lanes + C::kO + sm * DH;
     const uint32_t tw = tbase + lanes + C::kW + sm * C::kWCols;
-    const int lim = tile.r0 + row <= tile.last ? tile.seen(p, tile.r0 + row) : tile.n_keys;
+    float ref[4], l[4];
+    int lim[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int r = tile.r0 + row0 + 8 * y;
+      ref[y] = kNoRef;
+      l[y] = 0.0f;
+      lim[y] = r <= tile.last ? tile.seen(p, r) : tile.n_keys;
+    }
     int n = 0;
     bool ok = true;
     for (int i = sm; i < n_mine && ok; i += 2, ++n) {
-      const float* sc = sScale + (i % C::kStages) * 2 * KT;
-      const int k0 = (rank + p.C * i) * KT;
-      const bool masked = k0 + KT > tile.n_all;
+      const float* sc = sScale + (i % C::kStages) * 2 * KT + 2 * c4;
+      const int k0 = (rank + p.C * i) * KT + 2 * c4;
+      const bool masked = (rank + p.C * i) * KT + KT > tile.n_all;
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sm], n & 1, abort_flag, p.status, kDevTimeoutSoftmax));
       if (!ok) break;
       tc_fence_after();
       bool w_free = n == 0;  // the stream's previous product has read W
       for (int tries = 0;; ++tries) {
-        float big = 0.0f;
-        uint64_t sum = f2_pack(0.0f, 0.0f);
-        const uint64_t nref = f2_pack(-ref, -ref);
+        float big[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint64_t sum[4], nref[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          sum[y] = f2_pack(0.0f, 0.0f);
+          nref[y] = f2_pack(-ref[y], -ref[y]);
+        }
         // weights of columns c .. c + 31 against `ref` (a masked key's scale may be anything)
-        auto weigh = [&](int c, const uint32_t (&s)[32], auto mask) {
-          uint32_t w1[16], w2[kSplit ? 16 : 1];
+        auto weigh = [&](int c, const uint32_t (&s)[2][16], auto mask) {
+          uint32_t w[2][2][8];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const ulonglong2 ks = *reinterpret_cast<const ulonglong2*>(sc + c + j);
-            const ulonglong2 vs = *reinterpret_cast<const ulonglong2*>(sc + KT + c + j);
+          for (int g = 0; g < 4; ++g) {
+            const uint64_t ks = *reinterpret_cast<const uint64_t*>(sc + c + 8 * g);
+            const uint64_t vs = *reinterpret_cast<const uint64_t*>(sc + KT + c + 8 * g);
 #pragma unroll
-            for (int z = 0; z < 4; z += 2) {
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t* sy = &s[y >> 1][4 * g + 2 * (y & 1)];
               float d0, d1, x0, x1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(s[j + z]), __uint_as_float(s[j + z + 1])), z ? ks.y : ks.x, nref),
-                        d0, d1);
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(sy[0]), __uint_as_float(sy[1])), ks, nref[y]), d0, d1);
               float e0 = fast_exp2(d0), e1 = fast_exp2(d1);
-              const uint64_t e = f2_pack(e0, e1);
-              f2_unpack(f2_mul(e, z ? vs.y : vs.x), x0, x1);
+              f2_unpack(f2_mul(f2_pack(e0, e1), vs), x0, x1);
               if (mask) {
-                if (k0 + c + j + z >= lim) e0 = x0 = 0.0f;
-                if (k0 + c + j + z + 1 >= lim) e1 = x1 = 0.0f;
-                sum = f2_add(sum, f2_pack(e0, e1));
-              } else {
-                sum = f2_add(sum, e);
+                if (k0 + c + 8 * g >= lim[y]) e0 = x0 = 0.0f;
+                if (k0 + c + 8 * g + 1 >= lim[y]) e1 = x1 = 0.0f;
               }
-              big = max3f(big, fabsf(x0), fabsf(x1));
-              w1[(j + z) / 2] = half_pair(x0, x1);
-              if constexpr (kSplit) w2[(j + z) / 2] = half_rest(w1[(j + z) / 2], x0, x1);
+              sum[y] = f2_add(sum[y], f2_pack(e0, e1));
+              big[y] = max3f(big[y], fabsf(x0), fabsf(x1));
+              const uint32_t hi = half_pair(x0, x1);
+              w[0][y >> 1][2 * g + (y & 1)] = hi;
+              if constexpr (kSplit) w[1][y >> 1][2 * g + (y & 1)] = half_rest(hi, x0, x1);
             }
           }
           if (!w_free) {
@@ -317,19 +330,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_after();
             w_free = true;
           }
-          tmem_st_32x32b_x16(tw + c / 2, w1);
-          if constexpr (kSplit) tmem_st_32x32b_x16(tw + KT / 2 + c / 2, w2);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            tmem_st_16x128b_x4(tw + h * kHalf + c / 2, w[0][h]);
+            if constexpr (kSplit) tmem_st_16x128b_x4(tw + h * kHalf + KT / 2 + c / 2, w[1][h]);
+          }
+        };
+        auto load = [&](int c, uint32_t (&s)[2][16]) {
+          tmem_ld_16x256b_x4(ts + c, s[0]);
+          tmem_ld_16x256b_x4(ts + kHalf + c, s[1]);
         };
         auto pass = [&](auto mask) {
-          uint32_t s0[32], s1[32];
-          tmem_ld_32x32b_x32(ts, s0);
+          uint32_t s0[2][16], s1[2][16];
+          load(0, s0);
           tmem_ld_wait();
 #pragma unroll 1
           for (int c = 0; c < KT; c += 64) {
-            tmem_ld_32x32b_x32(ts + c + 32, s1);
+            load(c + 32, s1);
             weigh(c, s0, mask);
             tmem_ld_wait();
-            if (c + 64 < KT) tmem_ld_32x32b_x32(ts + c + 64, s0);
+            if (c + 64 < KT) load(c + 64, s0);
             weigh(c + 32, s1, mask);
             tmem_ld_wait();
           }
@@ -338,55 +358,89 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           pass(std::true_type{});
         else
           pass(std::false_type{});
-        float a, b;
-        f2_unpack(sum, a, b);
-        const float lu = l + (a + b);
-        const bool need = big >= kMaxWeight || lu >= kMaxSum;
+        float lu[4];
+        bool need = false;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          float a, b;
+          f2_unpack(sum[y], a, b);
+          lu[y] = l[y] + (a + b);
+          if (lu[y] >= kMaxSum) big[y] = INFINITY;
+          need = need || big[y] >= kMaxWeight;
+        }
         if (!ok || tries == 2 || !__any_sync(0xffffffffu, need)) {
-          l = lu;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) l[y] = lu[y];
           break;
         }
         // the references move, each by its own row's need only (a row that fits keeps its weights),
         // and the pass is repeated, twice at most (infinite scores or scales never fit).  A finite
         // overshoot says how far; the first tile, scores or scales far beyond, and a second try ask for
         // the maxima.
-        float moved = ref;
-        if (__any_sync(0xffffffffu, need && !(tries == 0 && big < 1e30f && lu < kMaxSum))) {
-          float top = -INFINITY, top_w = -INFINITY;
+        bool search = false;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 1));
+          big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 2));
+          search = search || (big[y] >= kMaxWeight && !(tries == 0 && big[y] < 1e30f));
+        }
+        float top[4], top_w[4];
+        search = __any_sync(0xffffffffu, search);
+        if (search) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) top[y] = top_w[y] = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < KT; c += 32) {
-            uint32_t s[32];
-            tmem_ld_32x32b_x32(ts + c, s);
+            uint32_t s[2][16];
+            load(c, s);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float x = k0 + c + j < lim ? __uint_as_float(s[j]) * sc[c + j] : -INFINITY;
-              top = fmaxf(top, x);
-              top_w = fmaxf(top_w, weight_log2(x, sc[KT + c + j]));
-            }
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const float ks = sc[c + 8 * g + z], lv = weight_log2(0.0f, sc[KT + c + 8 * g + z]);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const float x = k0 + c + 8 * g + z < lim[y]
+                                      ? __uint_as_float(s[y >> 1][4 * g + 2 * (y & 1) + z]) * ks
+                                      : -INFINITY;
+                  top[y] = fmaxf(top[y], x);
+                  top_w[y] = fmaxf(top_w[y], x + lv);
+                }
+              }
           }
-          if (need) moved = new_ref<T>(ref, top, top_w);
-        } else if (need) {
-          moved = ref + __log2f(big) - kTarget<T>;
         }
-        const float alpha = fast_exp2(ref - moved);
-        ref = moved;
-        l *= alpha;
+        float alpha[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          float moved = ref[y];
+          if (search) {
+#pragma unroll
+            for (int x = 1; x <= 2; x <<= 1) {
+              top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], x));
+              top_w[y] = fmaxf(top_w[y], __shfl_xor_sync(0xffffffffu, top_w[y], x));
+            }
+            if (big[y] >= kMaxWeight) moved = new_ref<T>(ref[y], top[y], top_w[y]);
+          } else if (big[y] >= kMaxWeight) {
+            moved = ref[y] + __log2f(big[y]) - kTarget<T>;
+          }
+          alpha[y] = fast_exp2(ref[y] - moved);
+          ref[y] = moved;
+          l[y] *= alpha[y];
+        }
         if (n > 0) {  // O *= alpha (the stream's previous product is complete)
-          const uint64_t a2 = f2_pack(alpha, alpha);
 #pragma unroll 1
           for (int c = 0; c < DH; c += 32) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(to + c, r);
-            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float x0, x1;
-              f2_unpack(f2_mul(f2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), a2), x0, x1);
-              r[j] = __float_as_uint(x0);
-              r[j + 1] = __float_as_uint(x1);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t r[16];
+              tmem_ld_16x256b_x4(to + h * kHalf + c, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha[2 * h + ((j >> 1) & 1)]);
+              tmem_st_16x256b_x4(to + h * kHalf + c, r);
             }
-            tmem_st_32x32b_x32(to + c, r);
           }
         }
       }
@@ -397,6 +451,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (ok && n > 0)
       __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
     tc_fence_after();
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+      l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+      if (c4 == 0) {
+        s_ref[sm * kRows + row0 + 8 * y] = ref[y];
+        s_l[sm * kRows + row0 + 8 * y] = l[y];
+      }
+    }
   }
   __syncthreads();  // every product is done: Q and the ring are free
 
@@ -416,8 +479,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int j = 0; j < 8; ++j)
         *reinterpret_cast<uint4*>(piece(row, c / 4 + j)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
     }
-    s_ref[row] = ref;
-    s_l[row] = l;
   }
   __syncthreads();
   // ---- A and B join (thread = row)
@@ -425,12 +486,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp < 4) {
     const int row = threadIdx.x;
     const uint32_t to = tbase + (static_cast<uint32_t>(warp * 32) << 16) + C::kO;
-    float M = ref, fa = 1.0f, fb = 0.0f, L = l;
+    float M = s_ref[row], fa = 1.0f, fb = 0.0f, L = s_l[row];
     if (two) {
-      M = fmaxf(ref, s_ref[row]);
-      fa = fast_exp2(ref - M);
-      fb = fast_exp2(s_ref[row] - M);
-      L = fmaf(fa, l, fb * s_l[row]);
+      const float ra = M, rb = s_ref[kRows + row];
+      M = fmaxf(ra, rb);
+      fa = fast_exp2(ra - M);
+      fb = fast_exp2(rb - M);
+      L = fmaf(fa, L, fb * s_l[kRows + row]);
     }
     const bool in = tile.r0 + row <= tile.last;
     T* dst = tile.out_row<T>(p, in ? tile.r0 + row : 0, DH);
@@ -472,8 +534,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
     if (!alone) {
-      s_ref[kRows + row] = M;
-      s_l[kRows + row] = L;
+      s_ref[row] = M;
+      s_l[row] = L;
     }
   }
   if (!alone) {
@@ -483,7 +545,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int i = rank * kTcThreads + static_cast<int>(threadIdx.x); i < n_rows * DH; i += p.C * kTcThreads) {
       const int row = i / DH, d = i % DH;
       const uint32_t a_o = smem_u32(piece(row, d >> 2) + (d & 3));
-      const uint32_t a_m = smem_u32(&s_ref[kRows + row]), a_l = smem_u32(&s_l[kRows + row]);
+      const uint32_t a_m = smem_u32(&s_ref[row]), a_l = smem_u32(&s_l[row]);
       float M = -INFINITY;
       for (int c = 0; c < p.C; ++c) M = fmaxf(M, ld_dsmem(a_m, c));
       float acc = 0.0f, L = 0.0f;
