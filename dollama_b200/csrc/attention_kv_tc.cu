@@ -1,20 +1,19 @@
 // Attention over the int8 K/V cache for many rows (prompt chunks), on tcgen05 (attention_kv.cu has
 // the formulas and the few-row kernel).
 //
-// One CTA takes 128 rows of one (sequence, kv head): row r is TMEM lane r.  Its key tiles (KT keys)
-// alternate between two streams A and B, each with its own scores, weights and output accumulator, so
-// that one stream's products run under the other's softmax; a cluster of C CTAs may share a tile's
-// keys.  All partial results meet at the end in a fixed order (A with B in the CTA, then the CTAs).
-//   warps 0..3 / 4..7   softmax of stream A / B: S from TMEM (32 columns at a time, the next ones
-//                       requested before the current ones are exponentiated), weights w = p vscale
-//                       against each row's running reference, as fp16 pairs into the stream's W
-//                       columns, from where the second product takes its A operand.  A lane takes
-//                       two of eight columns of four rows (the 16x256b pieces), so that a key's
-//                       scales, read from shared memory, serve four scores;
-//   warps 8 / 9         MMA issuers of A / B: S = Q K^T (M 128, N KT, K DH), O += W V (M 128,
-//                       N DH, K KT, V as an MN-major operand); the stream's next S is issued as soon
-//                       as the softmax is done with the last one, before W V;
-//   warps 10..13        the tiles' codes -> fp16 in the 128-byte-swizzled layout both products read,
+// One CTA takes 128 rows of one (sequence, kv head): row r is TMEM lane r.  Its tiles of 64 keys
+// alternate between two streams A and B, each with two score buffers and its own output accumulator,
+// so that a stream's next scores are there when the softmax comes to them, and one stream's
+// latencies lie under the other's softmax; a cluster of C CTAs may share a tile's keys.  All partial
+// results meet at the end in a fixed order (A with B in the CTA, then the CTAs).
+//   warps 0..3 / 4..7   softmax of stream A / B: S from TMEM, weights w = p vscale against each row's
+//                       running reference, as fp16 pairs back into S's columns, from where the second
+//                       product takes its A operand.  A lane takes two of eight columns of four rows
+//                       (the 16x256b pieces), so that a key's scales, read from shared memory, serve
+//                       four scores;
+//   warps 8 / 9         MMA issuers of A / B: S = Q K^T (M 128, N 64, K DH), O += W V (M 128, N DH,
+//                       K 64, V as an MN-major operand); a buffer's next S follows its W V;
+//   the other warps     the tiles' codes -> fp16 in the 128-byte-swizzled layout both products read,
 //                       with the tile's scales, through a ring of kStages tiles (the next tile's
 //                       codes are requested before the current one is converted).
 // The scales stay outside the products, as in the few-row kernel: codes are exact in fp16.  q is
@@ -32,22 +31,24 @@ constexpr int kRows = 128;
 constexpr int kConvWarps = 4;
 constexpr int kTcThreads = (8 + 2 + kConvWarps) * 32;
 
+constexpr int KT = 64;  // keys per tile
+
 template <int DH, bool kSplit>
 struct TcCfg {
-  static constexpr int KT = kSplit || DH == 128 ? 64 : 128;  // keys per tile
-  static constexpr int NT = kSplit ? 2 : 1;                  // fp16 terms of q and of the weights
-  static constexpr int kHalves = DH / 64;                    // 64-channel blocks (128-byte rows)
+  static constexpr int NT = kSplit ? 2 : 1;  // fp16 terms of q and of the weights
+  static constexpr int kHalves = DH / 64;    // 64-channel blocks (128-byte rows)
   static constexpr int kQBytes = NT * kHalves * kRows * 128;
   static constexpr int kTile = kHalves * KT * 128;  // K or V of a tile
-  static constexpr int kStages = kTile <= 8192 ? 4 : 3;
+  static constexpr int kStages = DH == 64 ? 6 : 4;
   static constexpr int kScales = 2 * KT * 4;  // kscale, vscale
   static constexpr int kRing = kStages * 2 * kTile;
   static constexpr int kOut = kRows * DH * 4;  // O of stream B, then the CTA's, over Q and the ring
   static constexpr int kData = kQBytes + kRing > kOut ? kQBytes + kRing : kOut;
   static constexpr int kSmem = kData + kStages * kScales + kRows * 4 * 4 + 512 + 1024;
-  // TMEM columns: S, O and W of the two streams
-  static constexpr uint32_t kS = 0, kO = 2 * KT, kW = kO + 2 * DH, kWCols = NT * KT / 2;
-  static_assert(kW + 2 * kWCols <= 512, "tensor memory");
+  // TMEM columns: two S buffers of each stream (the weights' terms replace the scores, KT / 2 columns
+  // each), then the streams' O
+  static constexpr uint32_t kO = 4 * KT;
+  static_assert(kO + 2 * DH <= 512 && NT * KT / 2 <= KT, "tensor memory");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr bool kSplit = sizeof(T) == 4;
   constexpr bool kScaled = !std::is_same<T, __half>::value;
   using C = TcCfg<DH, kSplit>;
-  constexpr int KT = C::KT, NT = C::NT;
+  constexpr int NT = C::NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -76,9 +77,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + 2 * kRows);
   uint64_t* kv_full = bars;                  // [stages]
   uint64_t* kv_empty = kv_full + C::kStages; // [stages]
-  uint64_t* s_full = kv_empty + C::kStages;  // [stream]
-  uint64_t* w_full = s_full + 2;             // [stream]
-  uint64_t* o_full = w_full + 2;             // [stream]
+  uint64_t* s_full = kv_empty + C::kStages;  // [stream][buffer]
+  uint64_t* w_full = s_full + 4;             // [stream][buffer]
+  uint64_t* o_full = w_full + 4;             // [stream]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_top = reinterpret_cast<float*>(tmem_slot + 2);  // [4] largest |q| of the four warps' rows
@@ -90,11 +91,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&kv_full[s], kConvWarps * 32);
       mbar_init(&kv_empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&w_full[s], kRows);
-      mbar_init(&o_full[s], 1);
     }
+    for (int s = 0; s < 2; ++s) mbar_init(&o_full[s], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -226,11 +227,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int sm = warp - 8;
       constexpr uint32_t idesc_s = idesc_f16_f32(kRows, KT, false);
       constexpr uint32_t idesc_o = idesc_f16_f32(kRows, DH, true);
-      const uint32_t ts = tbase + C::kS + sm * KT, to = tbase + C::kO + sm * DH;
-      const uint32_t tw = tbase + C::kW + sm * C::kWCols;
-      // S of the CTA's tile i, once its codes are there
-      auto scores = [&](int i) -> bool {
-        const int st = i % C::kStages;
+      const uint32_t to = tbase + C::kO + sm * DH;
+      const int n_own = (n_mine - sm + 1) / 2;  // tiles of this stream
+      // S of the stream's tile n (the CTA's tile 2 n + sm), once its codes are there
+      auto scores = [&](int n) -> bool {
+        const int i = 2 * n + sm, st = i % C::kStages;
         if (!mbar_wait(&kv_full[st], (i / C::kStages) & 1, abort_flag, p.status, kDevTimeoutMma)) return false;
         tc_fence_after();
         const uint32_t k_addr = smem_u32(sKV + st * 2 * C::kTile);
@@ -240,17 +241,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int h = 0; h < C::kHalves; ++h)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16_ss(ts, sw128_desc(smem_u32(sQ) + (x * C::kHalves + h) * kRows * 128 + k * 32, 16, 1024),
+              umma_f16_ss(tbase + (2 * sm + (n & 1)) * KT,
+                          sw128_desc(smem_u32(sQ) + (x * C::kHalves + h) * kRows * 128 + k * 32, 16, 1024),
                           sw128_desc(k_addr + h * KT * 128 + k * 32, 16, 1024), idesc_s,
                           (x | h | k) != 0 ? 1u : 0u);
-        umma_commit(&s_full[sm]);
+        umma_commit(&s_full[2 * sm + (n & 1)]);
         return true;
       };
-      bool ok = sm >= n_mine || scores(sm);
-      for (int i = sm, n = 0; ok && i < n_mine; i += 2, ++n) {
-        const int st = i % C::kStages;
-        ok = mbar_wait(&w_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma);
-        if (ok && i + 2 < n_mine) ok = scores(i + 2);  // the softmax is done with S
+      bool ok = (n_own < 1 || scores(0)) && (n_own < 2 || scores(1));
+      for (int n = 0; ok && n < n_own; ++n) {
+        const int st = (2 * n + sm) % C::kStages, buf = 2 * sm + (n & 1);
+        ok = mbar_wait(&w_full[buf], (n >> 1) & 1, abort_flag, p.status, kDevTimeoutMma);
         if (!ok) break;
         tc_fence_after();
         const uint32_t v_addr = smem_u32(sKV + st * 2 * C::kTile) + C::kTile;
@@ -258,10 +259,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int x = 0; x < NT; ++x)
 #pragma unroll
           for (int k = 0; k < KT / 16; ++k)
-            umma_f16_ts(to, tw + x * (KT / 2) + k * 8, sw128_desc(v_addr + k * 2048, KT * 128, 1024), idesc_o,
-                        (n | x | k) != 0 ? 1u : 0u);
+            umma_f16_ts(to, tbase + buf * KT + x * (KT / 2) + k * 8, sw128_desc(v_addr + k * 2048, KT * 128, 1024),
+                        idesc_o, (n | x | k) != 0 ? 1u : 0u);
         umma_commit(&kv_empty[st]);
         umma_commit(&o_full[sm]);
+        if (n + 2 < n_own) {
+          // the buffer's next scores replace the weights that this product reads
+          ok = mbar_wait(&o_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma) && scores(n + 2);
+        }
       }
       griddep_launch_dependents();
     }
@@ -271,8 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int row0 = (warp & 3) * 32 + gr;  // this lane's rows: row0 + 8 y
     constexpr uint32_t kHalf = 16u << 16;   // TMEM address of 16 lanes further
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tbase + lanes + C::kS + sm * KT, to = tbase + lanes + C::kO + sm * DH;
-    const uint32_t tw = tbase + lanes + C::kW + sm * C::kWCols;
+    const uint32_t to = tbase + lanes + C::kO + sm * DH;
     float ref[4], l[4];
     int lim[4];
 #pragma unroll
@@ -288,147 +292,131 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float* sc = sScale + (i % C::kStages) * 2 * KT + 2 * c4;
       const int k0 = (rank + p.C * i) * KT + 2 * c4;
       const bool masked = (rank + p.C * i) * KT + KT > tile.n_all;
-      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[sm], n & 1, abort_flag, p.status, kDevTimeoutSoftmax));
+      const int buf = 2 * sm + (n & 1);
+      const uint32_t ts = tbase + lanes + buf * KT;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], (n >> 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
       if (!ok) break;
       tc_fence_after();
-      bool w_free = n == 0;  // the stream's previous product has read W
-      for (int tries = 0;; ++tries) {
-        float big[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      uint32_t s[4][16];  // [column half][lane half]
+      auto load = [&]() {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) tmem_ld_16x256b_x4(ts + (h & 1) * kHalf + (h >> 1) * 32, s[h]);
+        tmem_ld_wait();
+      };
+      load();
+      uint32_t w[NT][4][8];
+      float big[4], lu[4];
+      // weights against `ref` (a masked key's scale may be anything)
+      auto weigh = [&](auto mask) {
         uint64_t sum[4], nref[4];
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
+          big[y] = 0.0f;
           sum[y] = f2_pack(0.0f, 0.0f);
           nref[y] = f2_pack(-ref[y], -ref[y]);
         }
-        // weights of columns c .. c + 31 against `ref` (a masked key's scale may be anything)
-        auto weigh = [&](int c, const uint32_t (&s)[2][16], auto mask) {
-          uint32_t w[2][2][8];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const uint64_t ks = *reinterpret_cast<const uint64_t*>(sc + c + 8 * g);
-            const uint64_t vs = *reinterpret_cast<const uint64_t*>(sc + KT + c + 8 * g);
+        for (int g = 0; g < 8; ++g) {
+          const uint64_t ks = *reinterpret_cast<const uint64_t*>(sc + 8 * g);
+          const uint64_t vs = *reinterpret_cast<const uint64_t*>(sc + KT + 8 * g);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint32_t* sy = &s[y >> 1][4 * g + 2 * (y & 1)];
-              float d0, d1, x0, x1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(sy[0]), __uint_as_float(sy[1])), ks, nref[y]), d0, d1);
-              float e0 = fast_exp2(d0), e1 = fast_exp2(d1);
-              f2_unpack(f2_mul(f2_pack(e0, e1), vs), x0, x1);
-              if (mask) {
-                if (k0 + c + 8 * g >= lim[y]) e0 = x0 = 0.0f;
-                if (k0 + c + 8 * g + 1 >= lim[y]) e1 = x1 = 0.0f;
-              }
-              sum[y] = f2_add(sum[y], f2_pack(e0, e1));
-              big[y] = max3f(big[y], fabsf(x0), fabsf(x1));
-              const uint32_t hi = half_pair(x0, x1);
-              w[0][y >> 1][2 * g + (y & 1)] = hi;
-              if constexpr (kSplit) w[1][y >> 1][2 * g + (y & 1)] = half_rest(hi, x0, x1);
+          for (int y = 0; y < 4; ++y) {
+            const int h = (g >> 2) * 2 + (y >> 1), j = 4 * (g & 3) + 2 * (y & 1);
+            float d0, d1, x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[h][j]), __uint_as_float(s[h][j + 1])), ks, nref[y]), d0, d1);
+            float e0 = fast_exp2(d0), e1 = fast_exp2(d1);
+            f2_unpack(f2_mul(f2_pack(e0, e1), vs), x0, x1);
+            if (mask) {
+              if (k0 + 8 * g >= lim[y]) e0 = x0 = 0.0f;
+              if (k0 + 8 * g + 1 >= lim[y]) e1 = x1 = 0.0f;
             }
+            sum[y] = f2_add(sum[y], f2_pack(e0, e1));
+            big[y] = max3f(big[y], fabsf(x0), fabsf(x1));
+            const uint32_t hi = half_pair(x0, x1);
+            w[0][h][2 * (g & 3) + (y & 1)] = hi;
+            if constexpr (kSplit) w[NT - 1][h][2 * (g & 3) + (y & 1)] = half_rest(hi, x0, x1);
           }
-          if (!w_free) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
-            tc_fence_after();
-            w_free = true;
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            tmem_st_16x128b_x4(tw + h * kHalf + c / 2, w[0][h]);
-            if constexpr (kSplit) tmem_st_16x128b_x4(tw + h * kHalf + KT / 2 + c / 2, w[1][h]);
-          }
-        };
-        auto load = [&](int c, uint32_t (&s)[2][16]) {
-          tmem_ld_16x256b_x4(ts + c, s[0]);
-          tmem_ld_16x256b_x4(ts + kHalf + c, s[1]);
-        };
-        auto pass = [&](auto mask) {
-          uint32_t s0[2][16], s1[2][16];
-          load(0, s0);
-          tmem_ld_wait();
-#pragma unroll 1
-          for (int c = 0; c < KT; c += 64) {
-            load(c + 32, s1);
-            weigh(c, s0, mask);
-            tmem_ld_wait();
-            if (c + 64 < KT) load(c + 64, s0);
-            weigh(c + 32, s1, mask);
-            tmem_ld_wait();
-          }
-        };
-        if (masked)
-          pass(std::true_type{});
-        else
-          pass(std::false_type{});
-        float lu[4];
-        bool need = false;
+        }
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           float a, b;
           f2_unpack(sum[y], a, b);
           lu[y] = l[y] + (a + b);
-          if (lu[y] >= kMaxSum) big[y] = INFINITY;
-          need = need || big[y] >= kMaxWeight;
         }
-        if (!ok || tries == 2 || !__any_sync(0xffffffffu, need)) {
+      };
+      // References move each by its own row's need only (a row that fits keeps its weights), and the
+      // tile is weighed again, twice at most (infinite scores or scales never fit).  A finite overshoot
+      // says how far; the first tile, scores or scales far beyond, and a second try ask for the maxima.
+      bool search = n == 0;
+      for (int tries = 0;; ++tries) {
+        if (!search) {
+          if (masked)
+            weigh(std::true_type{});
+          else
+            weigh(std::false_type{});
+          bool need = false;
 #pragma unroll
-          for (int y = 0; y < 4; ++y) l[y] = lu[y];
-          break;
-        }
-        // the references move, each by its own row's need only (a row that fits keeps its weights),
-        // and the pass is repeated, twice at most (infinite scores or scales never fit).  A finite
-        // overshoot says how far; the first tile, scores or scales far beyond, and a second try ask for
-        // the maxima.
-        bool search = false;
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 1));
-          big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 2));
-          search = search || (big[y] >= kMaxWeight && !(tries == 0 && big[y] < 1e30f));
-        }
-        float top[4], top_w[4];
-        search = __any_sync(0xffffffffu, search);
-        if (search) {
-#pragma unroll
-          for (int y = 0; y < 4; ++y) top[y] = top_w[y] = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < KT; c += 32) {
-            uint32_t s[2][16];
-            load(c, s);
-            tmem_ld_wait();
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                const float ks = sc[c + 8 * g + z], lv = weight_log2(0.0f, sc[KT + c + 8 * g + z]);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  const float x = k0 + c + 8 * g + z < lim[y]
-                                      ? __uint_as_float(s[y >> 1][4 * g + 2 * (y & 1) + z]) * ks
-                                      : -INFINITY;
-                  top[y] = fmaxf(top[y], x);
-                  top_w[y] = fmaxf(top_w[y], x + lv);
-                }
-              }
+          for (int y = 0; y < 4; ++y) {
+            if (lu[y] >= kMaxSum) big[y] = INFINITY;
+            need = need || big[y] >= kMaxWeight;
           }
+          if (tries == 2 || !__any_sync(0xffffffffu, need)) break;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 1));
+            big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 2));
+            search = search || (big[y] >= kMaxWeight && !(tries == 0 && big[y] < 1e30f));
+          }
+          search = __any_sync(0xffffffffu, search);
+          load();
+        } else {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) big[y] = INFINITY;
         }
         float alpha[4];
+        if (search) {
+          float top[4], top_w[4];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          float moved = ref[y];
-          if (search) {
+          for (int y = 0; y < 4; ++y) top[y] = top_w[y] = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 8; ++g)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const float ks = sc[8 * g + z], lv = weight_log2(0.0f, sc[KT + 8 * g + z]);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const float v = __uint_as_float(s[(g >> 2) * 2 + (y >> 1)][4 * (g & 3) + 2 * (y & 1) + z]);
+                const float x = k0 + 8 * g + z < lim[y] ? v * ks : -INFINITY;
+                top[y] = fmaxf(top[y], x);
+                top_w[y] = fmaxf(top_w[y], x + lv);
+              }
+            }
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
 #pragma unroll
             for (int x = 1; x <= 2; x <<= 1) {
               top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], x));
               top_w[y] = fmaxf(top_w[y], __shfl_xor_sync(0xffffffffu, top_w[y], x));
             }
-            if (big[y] >= kMaxWeight) moved = new_ref<T>(ref[y], top[y], top_w[y]);
-          } else if (big[y] >= kMaxWeight) {
-            moved = ref[y] + __log2f(big[y]) - kTarget<T>;
+            alpha[y] = big[y] >= kMaxWeight ? new_ref<T>(ref[y], top[y], top_w[y]) : ref[y];
           }
+        } else {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            alpha[y] = big[y] >= kMaxWeight ? ref[y] + __log2f(big[y]) - kTarget<T> : ref[y];
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float moved = alpha[y];
           alpha[y] = fast_exp2(ref[y] - moved);
           ref[y] = moved;
           l[y] *= alpha[y];
         }
-        if (n > 0) {  // O *= alpha (the stream's previous product is complete)
+        search = false;
+        if (n > 0) {  // O *= alpha, once the stream's previous product is in it
+          ok = __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < DH; c += 32) {
 #pragma unroll
@@ -444,9 +432,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
         }
       }
+      if (!ok) break;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) l[y] = lu[y];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          tmem_st_16x128b_x4(ts + (h & 1) * kHalf + x * (KT / 2) + (h >> 1) * 16, w[x][h]);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&w_full[sm]);
+      mbar_arrive(&w_full[buf]);
     }
     if (ok && n > 0)
       __all_sync(0xffffffffu, mbar_wait(&o_full[sm], (n - 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
@@ -591,9 +587,9 @@ int attn_kv_tc(const AttnKvParams& given, cudaStream_t s) {
   constexpr double kFixed = 512.0;
   double best = 1e30;
   for (int c = 1; c <= 8; ++c) {
-    const long long units = (p.Lmax + static_cast<long long>(C::KT) * c - 1) / (C::KT * c);
+    const long long units = (p.Lmax + static_cast<long long>(KT) * c - 1) / (KT * c);
     const double t = static_cast<double>((tiles * c + num_sms() - 1) / num_sms()) *
-                     (static_cast<double>(units * C::KT) + kFixed);
+                     (static_cast<double>(units * KT) + kFixed);
     if (t < 0.97 * best) {
       best = t;
       p.C = c;
