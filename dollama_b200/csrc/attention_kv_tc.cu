@@ -28,7 +28,7 @@ namespace dlm {
 namespace {
 
 constexpr int kRows = 128;
-constexpr int kConvWarps = 4;
+constexpr int kConvWarps = 2;  // (with four, a scheduler's share of the registers would be 128 a thread)
 constexpr int kTcThreads = (8 + 2 + kConvWarps) * 32;
 
 constexpr int KT = 64;  // keys per tile
@@ -171,7 +171,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const float* ksb = p.ks + head * p.Lmax;
     const float* vsb = p.vs + head * p.Lmax;
     uint4 rk[kEach], rv[kEach];
-    float sk = 0.0f, sv = 0.0f;
+    constexpr int kSc = KT / (kConvWarps * 32);  // keys whose scales a thread stages
+    float sk[kSc], sv[kSc];
     auto request = [&](int i) {
       const int k0 = (rank + p.C * i) * KT;
 #pragma unroll
@@ -182,9 +183,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         rk[e] = in ? __ldg(reinterpret_cast<const uint4*>(kb + off)) : make_uint4(0, 0, 0, 0);
         rv[e] = in ? __ldg(reinterpret_cast<const uint4*>(vb + off)) : make_uint4(0, 0, 0, 0);
       }
-      const bool in = t < KT && k0 + t < tile.n_keys;
-      sk = in ? __ldg(ksb + k0 + t) : 0.0f;
-      sv = in ? __ldg(vsb + k0 + t) : 0.0f;
+#pragma unroll
+      for (int e = 0; e < kSc; ++e) {
+        const int key = k0 + e * kConvWarps * 32 + t;
+        sk[e] = key < tile.n_keys ? __ldg(ksb + key) : 0.0f;
+        sv[e] = key < tile.n_keys ? __ldg(vsb + key) : 0.0f;
+      }
     };
     if (n_mine > 0) request(0);
     int st = 0;
@@ -209,9 +213,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         *reinterpret_cast<uint4*>(dv + off + p0) = odd ? b : a;
         *reinterpret_cast<uint4*>(dv + off + p1) = odd ? a : b;
       }
-      if (t < KT) {
-        sScale[st * 2 * KT + t] = sk * qmul;
-        sScale[st * 2 * KT + KT + t] = sv;
+#pragma unroll
+      for (int e = 0; e < kSc; ++e) {
+        sScale[st * 2 * KT + e * kConvWarps * 32 + t] = sk[e] * qmul;
+        sScale[st * 2 * KT + KT + e * kConvWarps * 32 + t] = sv[e];
       }
       if (i + 1 < n_mine) request(i + 1);
       fence_proxy_async_smem();
