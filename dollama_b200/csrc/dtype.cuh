@@ -27,11 +27,64 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// a * b + c in fp32 from two elements (the products of 16-bit elements are exact).
+template <typename T>
+__device__ __forceinline__ float fma_f(T a, T b, float c);
+template <>
+__device__ __forceinline__ float fma_f<float>(float a, float b, float c) { return fmaf(a, b, c); }
+template <>
+__device__ __forceinline__ float fma_f<__half>(__half a, __half b, float c) {
+  float d;
+  asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(d) : "h"(__half_as_ushort(a)), "h"(__half_as_ushort(b)), "f"(c));
+  return d;
+}
+template <>
+__device__ __forceinline__ float fma_f<__nv_bfloat16>(__nv_bfloat16 a, __nv_bfloat16 b, float c) {
+  float d;
+  asm("fma.rn.f32.bf16 %0, %1, %2, %3;"
+      : "=f"(d)
+      : "h"(__bfloat16_as_ushort(a)), "h"(__bfloat16_as_ushort(b)), "f"(c));
+  return d;
+}
+
 // N consecutive elements as one load or store of sizeof(T) * N <= 16 bytes.
 template <typename T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
+
+// a[j] += b[j], rounded once to T
+template <int N>
+__device__ __forceinline__ void add_to(Vec<float, N>& a, const Vec<float, N>& b) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) a.v[j] += b.v[j];
+}
+template <int N>
+__device__ __forceinline__ void add_to(Vec<__half, N>& a, const Vec<__half, N>& b) {
+  if constexpr (N == 1) {
+    a.v[0] = __hadd(a.v[0], b.v[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const __half2 s = __hadd2(__halves2half2(a.v[j], a.v[j + 1]), __halves2half2(b.v[j], b.v[j + 1]));
+      a.v[j] = __low2half(s);
+      a.v[j + 1] = __high2half(s);
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void add_to(Vec<__nv_bfloat16, N>& a, const Vec<__nv_bfloat16, N>& b) {
+  if constexpr (N == 1) {
+    a.v[0] = __hadd(a.v[0], b.v[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const __nv_bfloat162 s = __hadd2(__halves2bfloat162(a.v[j], a.v[j + 1]), __halves2bfloat162(b.v[j], b.v[j + 1]));
+      a.v[j] = __low2bfloat16(s);
+      a.v[j + 1] = __high2bfloat16(s);
+    }
+  }
+}
 
 // max that keeps a NaN of either operand
 __device__ __forceinline__ float max_nan(float a, float b) {

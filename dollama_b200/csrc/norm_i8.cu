@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
   T* ho = p.h ? static_cast<T*>(p.h) + static_cast<size_t>(row) * p.ldh : nullptr;
   extern __shared__ __align__(16) uint8_t s_row[];
   V h_reg[NV > 0 ? NV : 1];
+  float p_reg[NV > 0 ? NV : 1][VEC];  // h * w in fp32
   const int steps = NV > 0 ? NV : (p.K + blockDim.x * VEC - 1) / (blockDim.x * VEC);
   auto H = [&](int i) -> V& {
     if constexpr (NV > 0)
@@ -68,30 +69,36 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
   };
   float ss = 0.0f, amax = 0.0f;
   double damax = 0.0;
+  V r_reg[NV > 0 ? NV : 1];
 #pragma unroll(NV > 0 ? NV : 1)
   for (int i = 0; i < steps; ++i) {
     const int k = (i * blockDim.x + threadIdx.x) * VEC;
-    if (k < p.K) H(i) = *reinterpret_cast<const V*>(x + k);
+    if (k < p.K) {
+      H(i) = *reinterpret_cast<const V*>(x + k);
+      if constexpr (NV > 0)
+        if (r) r_reg[i] = *reinterpret_cast<const V*>(r + k);
+    }
   }
 #pragma unroll(NV > 0 ? NV : 1)
   for (int i = 0; i < steps; ++i) {
     const int k = (i * blockDim.x + threadIdx.x) * VEC;
     if (k >= p.K) continue;
+    V hv = H(i);
     if (r) {
-      const V rv = *reinterpret_cast<const V*>(r + k);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) H(i).v[j] = from_f<T>(to_f(H(i).v[j]) + to_f(rv.v[j]));
+      add_to(hv, NV > 0 ? r_reg[NV > 0 ? i : 0] : *reinterpret_cast<const V*>(r + k));
+      H(i) = hv;
     }
-    if (ho) *reinterpret_cast<V*>(ho + k) = H(i);
+    if (ho) *reinterpret_cast<V*>(ho + k) = hv;
     const V wv = *reinterpret_cast<const V*>(w + k);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const float f = to_f(H(i).v[j]);
-      ss = fmaf(f, f, ss);
+      ss = fma_f(hv.v[j], hv.v[j], ss);
+      const float f = fma_f(hv.v[j], wv.v[j], 0.0f);
+      if constexpr (NV > 0) p_reg[i][j] = f;
       if constexpr (kWide)
-        damax = max_nan_d(fabs(static_cast<double>(f) * static_cast<double>(to_f(wv.v[j]))), damax);
+        damax = max_nan_d(fabs(static_cast<double>(to_f(hv.v[j])) * static_cast<double>(to_f(wv.v[j]))), damax);
       else
-        amax = max_nan(amax, fabsf(f * to_f(wv.v[j])));
+        amax = max_nan(amax, fabsf(f));
     }
   }
   if constexpr (kWide) amax = static_cast<float>(damax);
@@ -173,10 +180,9 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
   for (int i = 0; i < steps; ++i) {
     const int k = (i * blockDim.x + threadIdx.x) * VEC;
     if (k >= p.K) continue;
-    const V wv = *reinterpret_cast<const V*>(w + k);
     const V hv = H(i);
     auto exact = [&](int j) {
-      return quant_exact(static_cast<double>(to_f(hv.v[j])) * static_cast<double>(to_f(wv.v[j])), damax);
+      return quant_exact(static_cast<double>(to_f(hv.v[j])) * static_cast<double>(to_f(w[k + j])), damax);
     };
     // 127 / a and its product: within 127 * 2^-23 for exact products and a, twice that otherwise
     constexpr float kErr = kWide ? 0x1p-14f : 0x1p-15f;
@@ -184,7 +190,12 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
     float v[N];
     uint32_t c[N / 4];
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = j < VEC ? to_f(hv.v[j < VEC ? j : 0]) * to_f(wv.v[j < VEC ? j : 0]) * rq : 0.0f;
+    for (int j = 0; j < N; ++j) {
+      if constexpr (NV > 0)
+        v[j] = p_reg[i][j] * rq;
+      else
+        v[j] = j < VEC ? fma_f(hv.v[j < VEC ? j : 0], w[k + (j < VEC ? j : 0)], 0.0f) * rq : 0.0f;
+    }
     if (plain) {
       quant_codes<N>(v, kErr, c, exact);
     } else {
