@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
   __shared__ double s_dsum[32], s_dmax[32];
   const int nw = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   using V = Vec<T, VEC>;
-  const T* w = static_cast<const T*>(p.w);
+  const T* __restrict__ w = static_cast<const T*>(p.w);
   const int row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + static_cast<size_t>(row) * p.ldx;
   const T* r = p.r ? static_cast<const T*>(p.r) + static_cast<size_t>(row) * p.ldr : nullptr;
@@ -176,25 +176,32 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
                          : static_cast<float>(dscale);
   const float rq = 127.0f / amax;
   int8_t* qo = p.q + static_cast<size_t>(row) * p.K;
+  // 127 / a and its product: within 127 * 2^-23 for exact products and a, twice that otherwise
+  constexpr float kErr = kWide ? 0x1p-14f : 0x1p-15f;
+  // codes of N values at a time: of one vector, or (VEC == 1) of four steps
+  constexpr int N = VEC == 1 ? 4 : VEC, kStep = VEC == 1 ? 4 : 1;
 #pragma unroll(NV > 0 ? NV : 1)
-  for (int i = 0; i < steps; ++i) {
-    const int k = (i * blockDim.x + threadIdx.x) * VEC;
-    if (k >= p.K) continue;
-    const V hv = H(i);
-    auto exact = [&](int j) {
-      return quant_exact(static_cast<double>(to_f(hv.v[j])) * static_cast<double>(to_f(w[k + j])), damax);
+  for (int i = 0; i < steps; i += kStep) {
+    // value j of the N: its step, its place in the row
+    auto step = [&](int j) { return VEC == 1 ? i + j : i; };
+    auto at = [&](int j) {
+      return VEC == 1 ? (i + j) * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)
+                      : (i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * VEC + j;
     };
-    // 127 / a and its product: within 127 * 2^-23 for exact products and a, twice that otherwise
-    constexpr float kErr = kWide ? 0x1p-14f : 0x1p-15f;
-    constexpr int N = VEC < 4 ? 4 : VEC;
+    if (at(0) >= p.K) continue;
+    auto exact = [&](int j) {
+      const T hj = H(step(j)).v[VEC == 1 ? 0 : j];
+      return quant_exact(static_cast<double>(to_f(hj)) * static_cast<double>(to_f(w[at(j)])), damax);
+    };
     float v[N];
     uint32_t c[N / 4];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
+      const bool in = VEC > 1 || at(j) < p.K;
       if constexpr (NV > 0)
-        v[j] = p_reg[i][j] * rq;
+        v[j] = in ? p_reg[step(j)][VEC == 1 ? 0 : j] * rq : 0.0f;
       else
-        v[j] = j < VEC ? fma_f(hv.v[j < VEC ? j : 0], w[k + (j < VEC ? j : 0)], 0.0f) * rq : 0.0f;
+        v[j] = in ? fma_f(H(step(j)).v[VEC == 1 ? 0 : j], w[at(j)], 0.0f) * rq : 0.0f;
     }
     if (plain) {
       quant_codes<N>(v, kErr, c, exact);
@@ -202,16 +209,20 @@ __global__ void __launch_bounds__(kNormMaxThreads<NV>) add_rms_norm_i8_kernel(co
       const bool some = damax > 0.0 && dscale == dscale;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const uint32_t code = j < VEC && some ? static_cast<uint32_t>(exact(j < VEC ? j : 0)) & 0xFFu : 0u;
+        const bool in = some && (VEC > 1 || at(j) < p.K);
+        const uint32_t code = in ? static_cast<uint32_t>(exact(j)) & 0xFFu : 0u;
         c[j / 4] = (j % 4 ? c[j / 4] : 0u) | code << (8 * (j % 4));
       }
     }
-    if constexpr (VEC < 4)
-      qo[k] = static_cast<int8_t>(c[0] & 0xFFu);
-    else if constexpr (VEC == 4)
-      *reinterpret_cast<uint32_t*>(qo + k) = c[0];
-    else
-      *reinterpret_cast<uint2*>(qo + k) = make_uint2(c[0], c[1]);
+    if constexpr (VEC == 1) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (at(j) < p.K) qo[at(j)] = static_cast<int8_t>(c[0] >> (8 * j) & 0xFFu);
+    } else if constexpr (VEC == 4) {
+      *reinterpret_cast<uint32_t*>(qo + at(0)) = c[0];
+    } else {
+      *reinterpret_cast<uint2*>(qo + at(0)) = make_uint2(c[0], c[1]);
+    }
   }
 }
 
@@ -222,7 +233,9 @@ int launch_norm(const NormParams& p, cudaStream_t s) {
     const int threads = ((n + nv - 1) / nv + 31) / 32 * 32;
     return launch_pdl(kernel, dim3(p.M), dim3(threads), 0, s, p);
   };
-  if (VEC > 1 && n <= 256) {
+  if (VEC == 1 && n <= 4096) {
+    DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, (VEC == 1 ? 8 : 0)>, 8));
+  } else if (VEC > 1 && n <= 256) {
     DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, (VEC > 1 ? 1 : 0)>, 1));
   } else if (VEC > 1 && n <= 512) {
     DLM_CHECK_CUDA(go(add_rms_norm_i8_kernel<T, VEC, (VEC > 1 ? 2 : 0)>, 2));
