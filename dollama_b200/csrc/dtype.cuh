@@ -93,6 +93,28 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// max_j |x_j|, NaN if any is
+template <int N>
+__device__ __forceinline__ float max_abs(const Vec<float, N>& x, float m) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) m = max_nan(m, fabsf(x.v[j]));
+  return m;
+}
+template <int N>
+__device__ __forceinline__ float max_abs(const Vec<__half, N>& x, float m) {
+  __half2 t = __habs2(__halves2half2(x.v[0], x.v[1]));
+#pragma unroll
+  for (int j = 2; j < N; j += 2) t = __hmax2_nan(t, __habs2(__halves2half2(x.v[j], x.v[j + 1])));
+  return max_nan(m, __half2float(__hmax_nan(__low2half(t), __high2half(t))));
+}
+template <int N>
+__device__ __forceinline__ float max_abs(const Vec<__nv_bfloat16, N>& x, float m) {
+  __nv_bfloat162 t = __habs2(__halves2bfloat162(x.v[0], x.v[1]));
+#pragma unroll
+  for (int j = 2; j < N; j += 2) t = __hmax2_nan(t, __habs2(__halves2bfloat162(x.v[j], x.v[j + 1])));
+  return max_nan(m, __bfloat162float(__hmax_nan(__low2bfloat16(t), __high2bfloat16(t))));
+}
+
 // The absmax int8 codes round_half_away(127 x_j / a) of N values (a multiple of 4) of a row of
 // largest magnitude a, given v_j = x_j * (127 / a) in fp32, which is within `err` of the quotient:
 // away from a half-integer v_j rounds as the quotient does.  Next to one `exact(j)` forms the
@@ -115,6 +137,22 @@ __device__ __forceinline__ void quant_codes(const float (&v)[N], float err, uint
       if (fabsf(__fsub_rn(v[j], __fsub_rn(__uint_as_float(t[j]), kMagic))) >= 0.5f - err)
         t[j] = static_cast<uint32_t>(exact(j));
   }
+#pragma unroll
+  for (int j = 0; j < N; j += 4)
+    out[j / 4] = __byte_perm(__byte_perm(t[j], t[j + 1], 0x0040), __byte_perm(t[j + 2], t[j + 3], 0x0040), 0x5410);
+}
+
+// The codes of N values x_j of a 16-bit type in a row of largest magnitude a, from v_j = x_j * r in fp32
+// with r = (127 / a) (1 + 2^-21), without a check: with integers x = m 2^s, a = n 2^s (m < 2^11, as
+// |x| <= a), the quotient 127 m / n is a half-integer or differs from every one by a fraction of at
+// least 1 / (254 m) > 2^-19 of itself.  The three roundings of v_j move it by less than 2^-22, so the
+// factor lies in (1, 1 + 2^-20): exact halves go away from zero, nothing else crosses one.
+constexpr float kHalvesAway = 1.0f + 0x1p-21f;
+template <int N>
+__device__ __forceinline__ void quant_codes_16(const float (&v)[N], uint32_t (&out)[N / 4]) {
+  uint32_t t[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) t[j] = __float_as_uint(__fadd_rn(v[j], 12582912.0f));
 #pragma unroll
   for (int j = 0; j < N; j += 4)
     out[j / 4] = __byte_perm(__byte_perm(t[j], t[j + 1], 0x0040), __byte_perm(t[j + 2], t[j + 3], 0x0040), 0x5410);

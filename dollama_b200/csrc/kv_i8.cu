@@ -80,11 +80,15 @@ __device__ __forceinline__ void write_row(Oct<T>& x, float a, int8_t* q, float* 
   auto exact = [&](int j) { return quant_exact(static_cast<double>(to_f(x.at(j))), da); };
   uint32_t c[2] = {0, 0};
   if (a >= 1e-30f && finite) {
-    const float rq = 127.0f / a;
+    constexpr bool k16 = sizeof(T) == 2;
+    const float rq = 127.0f / a * (k16 ? kHalvesAway : 1.0f);
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = to_f(x.at(j)) * rq;
-    quant_codes<8>(v, 0x1p-15f, c, exact);  // two roundings: within 127 * 2^-23
+    if constexpr (k16)
+      quant_codes_16<8>(v, c);
+    else
+      quant_codes<8>(v, 0x1p-15f, c, exact);  // two roundings: within 127 * 2^-23
   } else if (a > 0.0f && finite) {
     // 127 / a may leave fp32's range
 #pragma unroll
@@ -113,9 +117,9 @@ __global__ void __launch_bounds__(kKvThreads)
     xk.load(k + tok * ldk + hd * DH + c * 8);
     xv.load(v + tok * ldv + hd * DH + c * 8);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      ak = max_nan(ak, fabsf(to_f(xk.at(j))));
-      av = max_nan(av, fabsf(to_f(xv.at(j))));
+    for (int j = 0; j < Oct<T>::kPieces; ++j) {
+      ak = max_abs(xk.v[j], ak);
+      av = max_abs(xv.v[j], av);
     }
   }
 #pragma unroll

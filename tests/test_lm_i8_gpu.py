@@ -283,6 +283,27 @@ def test_cache_write_and_read(t, B, S, H, Dh, Lm, ragged):
         assert torch.equal(out.nan_to_num(nan=-5.0), wo.nan_to_num(nan=-5.0))
 
 
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_cache_codes_of_every_pair_of_mantissas(t):
+    """Every mantissa against every largest one, at exponent distances 0 to 8: codes exact, halves away
+    from zero."""
+    bits = 10 if t == F16 else 7
+    n = 1 << bits
+    m = (torch.arange(n, device="cuda", dtype=torch.float64) + n) / n  # [1, 2)
+    for d in range(9):
+        x = (m * 2.0 ** -d).repeat(n, 1)  # row: all mantissas, under one largest value
+        x = torch.where(x > m[:, None], -x / 2, x)
+        pad = -x.numel() // n % 60 if n % 60 == 0 else 60 - n % 60
+        x = torch.cat([x, x[:, :pad]], 1).view(n, -1, 60)
+        top = m[:, None, None].expand(-1, x.shape[1], 4)
+        k = torch.cat([x, top], 2).to(O.TYPES[t]).view(1, -1, 1, 64)
+        L_ = k.shape[1]
+        cache = empty_cache(1, 1, L_, 64)
+        append(k, k, cache, torch.zeros(1, dtype=torch.int32, device="cuda"), None, t, L_)
+        q, s = O.quant_rows(k)
+        assert torch.equal(cache[0].view(-1, 64), q.view(-1, 64)) and torch.equal(cache[1].view(-1), s.float().view(-1))
+
+
 def test_cache_positions_outside_are_skipped_and_reported():
     B, S, H, Dh, Lm = 4, 3, 2, 64, 8
     k = torch.randn(B, S, H, Dh, device="cuda")
