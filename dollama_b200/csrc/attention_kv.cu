@@ -37,15 +37,20 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 32;  // keys a warp takes at a time
 
-// NR: tiles of 8 rows
-template <int DH, int NR>
+// NR: tiles of 8 rows; ST: units of a warp's ring (the copies in flight), more of them where the grid
+// leaves an SM one CTA: with two, a warp that takes 16 units of one sequence's keys waits for each.
+template <int DH, int NR, int ST>
 struct Cfg {
-  static constexpr int kStages = DH == 64 ? 3 : 2;
   static constexpr int kStage = kUnit * (2 * DH + 8);  // K, V codes, two scales
-  static constexpr int kWarpBytes = kStages * kStage;
+  static constexpr int kWarpBytes = ST * kStage;
   static constexpr int kSmem = kWarps * kWarpBytes;
   static_assert(kWarpBytes >= 8 * NR * DH * 4, "a warp's partial result reuses its ring");
 };
+template <int DH>
+constexpr int kShallow = DH == 64 ? 3 : 2;
+template <int DH>
+constexpr int kDeep = DH == 64 ? 8 : 5;
+constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -74,10 +79,10 @@ __device__ __forceinline__ int swz(int r, int ch) {
   return m * 128 + (((r ^ m) & 1) << 6) + ((ch ^ (m & 2)) << 4);
 }
 
-template <typename T, int DH, int NR, bool kSolo>
+template <typename T, int DH, int NR, int ST, bool kSolo>
 __global__ void __launch_bounds__(kThreads)
     attn_kv_kernel(const AttnKvParams p) {
-  using C = Cfg<DH, NR>;
+  using C = Cfg<DH, NR, ST>;
   constexpr int kRows = 8 * NR;
   constexpr bool kSplit = sizeof(T) == 4;                    // two fp16 terms for q and the weights
   constexpr bool kScaled = !std::is_same<T, __half>::value;  // q scaled into fp16's range
@@ -149,7 +154,7 @@ __global__ void __launch_bounds__(kThreads)
     cp_async_commit();
   };
   int k_next = first;
-  for (int i = 0; i < C::kStages - 1; ++i, k_next += stride) fetch(k_next, i);
+  for (int i = 0; i < ST - 1; ++i, k_next += stride) fetch(k_next, i);
 
   // ---- q, the B operand: row gr, channels 64 h + 16 c4 + 4 z + {0, 1 | 2, 3} in k-step 4 h + z
   uint32_t qf[NT][NR][KS][2];
@@ -214,8 +219,8 @@ __global__ void __launch_bounds__(kThreads)
 
   int st = 0;
   for (int k0 = first; k0 < n_keys; k0 += stride, k_next += stride) {
-    fetch(k_next, st == 0 ? C::kStages - 1 : st - 1);
-    asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+    fetch(k_next, st == 0 ? ST - 1 : st - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
     __syncwarp();
     const uint8_t* sk = ring + st * C::kStage;
     const float* sks = reinterpret_cast<const float*>(sk + 2 * kUnit * DH) + gr;
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
-    if (++st == C::kStages) st = 0;
+    if (++st == ST) st = 0;
     __syncwarp();  // every lane is done with the stage before its next fetch
   }
   cp_async_wait_all();
@@ -415,7 +420,8 @@ __global__ void __launch_bounds__(kThreads)
   // ---- the CTA's warps join, element by element (each read and written by one thread)
   s_o = reinterpret_cast<float*>(s_ring);
   constexpr int kWarpFloats = C::kWarpBytes / 4;
-  for (int i = threadIdx.x; i < kRows * DH; i += kThreads) {
+  const int n_rows = last - r0 + 1;  // rows of this tile that exist
+  for (int i = threadIdx.x; i < n_rows * DH; i += kThreads) {
     const int r = i / DH;
     float M = s_m[0][r];
 #pragma unroll
@@ -427,34 +433,40 @@ __global__ void __launch_bounds__(kThreads)
       acc = fmaf(f, s_o[w * kWarpFloats + i], acc);
       ls = fmaf(f, s_l[w][r], ls);
     }
+    if (p.C == 1) {
+      tile.out_row<T>(p, r0 + r, DH)[i % DH] = from_f<T>(ls == 0.0f ? 0.0f : acc / ls);
+      continue;
+    }
     s_o[i] = acc;
     if (i % DH == 0) {
       s_cm[r] = M;
       s_cl[r] = ls;
     }
   }
-  auto store = [&](int r, int d, float v) { tile.out_row<T>(p, r0 + r, DH)[d] = from_f<T>(v); };
-  const int n_rows = last - r0 + 1;  // rows of this tile that exist
-  if (p.C == 1) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_rows * DH; i += kThreads) {
-      const float L = s_cl[i / DH];
-      store(i / DH, i % DH, L == 0.0f ? 0.0f : s_o[i] / L);
-    }
-    return;
-  }
+  if (p.C == 1) return;
   cluster_sync_all();
   for (int i = rank * kThreads + threadIdx.x; i < n_rows * DH; i += p.C * kThreads) {
     const int r = i / DH;
-    float M = -INFINITY;
-    for (int c = 0; c < p.C; ++c) M = fmaxf(M, ld_dsmem(smem_u32(&s_cm[r]), c));
-    float acc = 0.0f, L = 0.0f;
-    for (int c = 0; c < p.C; ++c) {
-      const float f = fast_exp2(ld_dsmem(smem_u32(&s_cm[r]), c) - M);
-      acc = fmaf(f, ld_dsmem(smem_u32(&s_o[i]), c), acc);
-      L = fmaf(f, ld_dsmem(smem_u32(&s_cl[r]), c), L);
-    }
-    store(r, i % DH, L == 0.0f ? 0.0f : acc / L);
+    // every CTA's three values are requested before any is used
+    float m[kMaxCluster], l[kMaxCluster], v[kMaxCluster], M = kNoRef, acc = 0.0f, L = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c)
+      if (c < p.C) {
+        m[c] = ld_dsmem(smem_u32(&s_cm[r]), c);
+        l[c] = ld_dsmem(smem_u32(&s_cl[r]), c);
+        v[c] = ld_dsmem(smem_u32(&s_o[i]), c);
+      }
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c)
+      if (c < p.C) M = fmaxf(M, m[c]);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c)
+      if (c < p.C) {
+        const float f = fast_exp2(m[c] - M);
+        acc = fmaf(f, v[c], acc);
+        L = fmaf(f, l[c], L);
+      }
+    tile.out_row<T>(p, r0 + r, DH)[i % DH] = from_f<T>(L == 0.0f ? 0.0f : acc / L);
   }
   cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
@@ -475,41 +487,50 @@ int residency(K kernel, int smem, int (&cache)[64], int& per_sm) {
 
 template <typename T, int DH, int NR>
 int launch(AttnKvParams p, cudaStream_t s) {
-  using C = Cfg<DH, NR>;
-  static int cache[2][64] = {{0}};
-  int per_sm = 0, per_sm_solo = 0;
-  int rc = residency(attn_kv_kernel<T, DH, NR, false>, C::kSmem, cache[0], per_sm);
-  if (rc == DLM_OK) rc = residency(attn_kv_kernel<T, DH, NR, true>, C::kSmem, cache[1], per_sm_solo);
+  using Few = Cfg<DH, NR, kDeep<DH>>;
+  using Many = Cfg<DH, NR, kShallow<DH>>;
+  auto many = attn_kv_kernel<T, DH, NR, kShallow<DH>, false>;
+  auto few = attn_kv_kernel<T, DH, NR, kDeep<DH>, false>;
+  auto solo = attn_kv_kernel<T, DH, NR, kShallow<DH>, true>;
+  static int cache[3][64] = {{0}};
+  int per_many = 0, per_few = 0, per_solo = 0;
+  int rc = residency(many, Many::kSmem, cache[0], per_many);
+  if (rc == DLM_OK) rc = residency(few, Few::kSmem, cache[1], per_few);
+  if (rc == DLM_OK) rc = residency(solo, Many::kSmem, cache[2], per_solo);
   if (rc != DLM_OK) return rc;
   const long long row_tiles = (static_cast<long long>(p.Sq) * p.g + 8 * NR - 1) / (8 * NR);
   const long long tiles = row_tiles * p.B * p.Hkv;
-  DLM_REQUIRE(tiles < (1ll << 27), DLM_ERR_UNSUPPORTED, "attention_kv_i8: too many rows");
+  DLM_REQUIRE(tiles < (1ll << 26), DLM_ERR_UNSUPPORTED, "attention_kv_i8: too many rows");
   p.row_tiles = static_cast<int>(row_tiles);
   p.tiles = static_cast<int>(tiles);
   // Waves times keys of a warp (plus its fixed work, about as long as kFixed keys), for one warp per
-  // tile and for clusters of 1 to 8 CTAs per tile.
+  // tile and for clusters of 1 to 8 CTAs per tile (a cluster of 16, which needs
+  // the kernel's leave, cost 7 us more to launch than it saved).
   constexpr double kFixed = 100.0;
   auto cost = [&](long long ctas, int resident, int warps) {
     const long long slots = static_cast<long long>(resident) * num_sms();
     const long long units = (p.Lmax + static_cast<long long>(kUnit) * warps - 1) / (kUnit * warps);
     return static_cast<double>((ctas + slots - 1) / slots) * (static_cast<double>(units * kUnit) + kFixed);
   };
-  double best = cost((tiles + kWarps - 1) / kWarps, per_sm_solo, 1);
+  const long long solo_ctas = (tiles + kWarps - 1) / kWarps;
+  double best = cost(solo_ctas, per_solo, 1);
   p.C = 0;
-  for (int c = 1; c <= 8; ++c) {
-    const double t = cost(tiles * c, per_sm, c * kWarps);
+  for (int c = 1; c <= kMaxCluster; ++c) {
+    const double t = cost(tiles * c, per_many, c * kWarps);
     if (t < 0.97 * best) {
       best = t;
       p.C = c;
     }
   }
   if (p.C == 0) {
-    DLM_CHECK_CUDA(launch_pdl(attn_kv_kernel<T, DH, NR, true>, dim3(static_cast<unsigned>((tiles + kWarps - 1) / kWarps)),
-                              dim3(kThreads), C::kSmem, s, p));
+    DLM_CHECK_CUDA(launch_pdl(solo, dim3(static_cast<unsigned>(solo_ctas)), dim3(kThreads), Many::kSmem, s, p));
     return DLM_OK;
   }
-  DLM_CHECK_CUDA(launch_clusters(attn_kv_kernel<T, DH, NR, false>, static_cast<unsigned>(tiles * p.C), kThreads,
-                                 C::kSmem, p.C, s, p));
+  const unsigned grid = static_cast<unsigned>(tiles * p.C);
+  if (static_cast<long long>(grid) <= static_cast<long long>(per_few) * num_sms())
+    DLM_CHECK_CUDA(launch_clusters(few, grid, kThreads, Few::kSmem, p.C, s, p));
+  else
+    DLM_CHECK_CUDA(launch_clusters(many, grid, kThreads, Many::kSmem, p.C, s, p));
   return DLM_OK;
 }
 
