@@ -28,8 +28,12 @@ namespace dlm {
 namespace {
 
 constexpr int kRows = 128;
-constexpr int kConvWarps = 2;  // (with four, a scheduler's share of the registers would be 128 a thread)
-constexpr int kTcThreads = (8 + 2 + kConvWarps) * 32;
+constexpr int kTcThreads = 512;  // 4 warpgroups: softmax A, softmax B, MMA issuers, conversion
+// Registers a thread of each warpgroup (launched with 128 each): what the issuers and the conversion
+// give back goes to the softmax, whose scores and weights of a tile stay in registers.
+constexpr int kRegsSoftmax = 168, kRegsIssue = 64, kRegsConvert = 112;
+static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsConvert <= 4 * 128, "the register split");
+constexpr int kConvThreads = 128;
 
 constexpr int KT = 64;  // keys per tile
 
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int rank = static_cast<int>(blockIdx.x % p.C);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&kv_full[s], kConvWarps * 32);
+      mbar_init(&kv_full[s], kConvThreads);
       mbar_init(&kv_empty[s], 1);
     }
     for (int s = 0; s < 4; ++s) {
@@ -160,35 +164,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
 
-  if (warp >= 10) {
+  // Every warp meets here once it has its registers: a warpgroup that is done at once (no keys) must not
+  // take back what the softmax is still waiting for.
+  auto split_done = [] { asm volatile("bar.sync 1, 512;" ::: "memory"); };
+  if (warp >= 12) {
     // ================================================================ codes -> fp16
-    const int t = threadIdx.x - 320;
-    constexpr int kPieces = DH / 16;                      // 16-code pieces of a row
-    constexpr int kEach = KT * kPieces / (kConvWarps * 32);  // pieces a thread converts, of K and of V
+    regs_dec<kRegsConvert>();
+    split_done();
+    const int t = threadIdx.x - 384;
+    constexpr int kPieces = DH / 16;                    // 16-code pieces of a row
+    constexpr int kEach = KT * kPieces / kConvThreads;  // pieces a thread converts, of K and of V
     const size_t head = tile.head(p);
     const int8_t* kb = p.kq + head * p.Lmax * DH;
     const int8_t* vb = p.vq + head * p.Lmax * DH;
     const float* ksb = p.ks + head * p.Lmax;
     const float* vsb = p.vs + head * p.Lmax;
     uint4 rk[kEach], rv[kEach];
-    constexpr int kSc = KT / (kConvWarps * 32);  // keys whose scales a thread stages
-    float sk[kSc], sv[kSc];
+    float sk = 0.0f, sv = 0.0f;
     auto request = [&](int i) {
       const int k0 = (rank + p.C * i) * KT;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
-        const int id = e * kConvWarps * 32 + t;
+        const int id = e * kConvThreads + t;
         const bool in = k0 + id / kPieces < tile.n_keys;
         const size_t off = static_cast<size_t>(k0) * DH + static_cast<size_t>(id) * 16;
         rk[e] = in ? __ldg(reinterpret_cast<const uint4*>(kb + off)) : make_uint4(0, 0, 0, 0);
         rv[e] = in ? __ldg(reinterpret_cast<const uint4*>(vb + off)) : make_uint4(0, 0, 0, 0);
       }
-#pragma unroll
-      for (int e = 0; e < kSc; ++e) {
-        const int key = k0 + e * kConvWarps * 32 + t;
-        sk[e] = key < tile.n_keys ? __ldg(ksb + key) : 0.0f;
-        sv[e] = key < tile.n_keys ? __ldg(vsb + key) : 0.0f;
-      }
+      const bool in = t < KT && k0 + t < tile.n_keys;
+      sk = in ? __ldg(ksb + k0 + t) : 0.0f;
+      sv = in ? __ldg(vsb + k0 + t) : 0.0f;
     };
     if (n_mine > 0) request(0);
     int st = 0;
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint8_t* dv = dk + C::kTile;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
-        const int id = e * kConvWarps * 32 + t;
+        const int id = e * kConvThreads + t;
         const int r = id / kPieces, ch = id % kPieces;
         // the second half's pieces go in the other order: no bank conflict with the first half's
         const int odd = DH == 128 ? ch >> 2 : 0;
@@ -213,10 +218,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         *reinterpret_cast<uint4*>(dv + off + p0) = odd ? b : a;
         *reinterpret_cast<uint4*>(dv + off + p1) = odd ? a : b;
       }
-#pragma unroll
-      for (int e = 0; e < kSc; ++e) {
-        sScale[st * 2 * KT + e * kConvWarps * 32 + t] = sk[e] * qmul;
-        sScale[st * 2 * KT + KT + e * kConvWarps * 32 + t] = sv[e];
+      if (t < KT) {
+        sScale[st * 2 * KT + t] = sk * qmul;
+        sScale[st * 2 * KT + KT + t] = sv;
       }
       if (i + 1 < n_mine) request(i + 1);
       fence_proxy_async_smem();
@@ -226,9 +230,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ph ^= 1;
       }
     }
+    __syncwarp();
+    regs_inc<128>();
   } else if (warp >= 8) {
     // ================================================================ MMA issuer of one stream
-    if (lane == 0) {
+    regs_dec<kRegsIssue>();
+    split_done();
+    if (lane == 0 && warp < 10) {
       const int sm = warp - 8;
       constexpr uint32_t idesc_s = idesc_f16_f32(kRows, KT, false);
       constexpr uint32_t idesc_o = idesc_f16_f32(kRows, DH, true);
@@ -275,8 +283,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       griddep_launch_dependents();
     }
+    __syncwarp();
+    regs_inc<128>();
   } else {
     // ================================================================ softmax of one stream
+    regs_inc<kRegsSoftmax>();
+    split_done();
     const int sm = warp >> 2, gr = lane >> 2, c4 = lane & 3;
     const int row0 = (warp & 3) * 32 + gr;  // this lane's rows: row0 + 8 y
     constexpr uint32_t kHalf = 16u << 16;   // TMEM address of 16 lanes further
@@ -461,6 +473,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         s_l[sm * kRows + row0 + 8 * y] = l[y];
       }
     }
+    __syncwarp();
+    regs_dec<128>();  // what follows runs with an even split again
   }
   __syncthreads();  // every product is done: Q and the ring are free
 
