@@ -236,50 +236,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ================================================================ MMA issuer of one stream
     regs_dec<kRegsIssue>();
     split_done();
-    if (lane == 0 && warp < 10) {
-      const int sm = warp - 8;
+    const int sm = __shfl_sync(0xffffffffu, warp, 0) - 8;
+    if (sm < 2) {
       constexpr uint32_t idesc_s = idesc_f16_f32(kRows, KT, false);
       constexpr uint32_t idesc_o = idesc_f16_f32(kRows, DH, true);
       const uint32_t to = tbase + C::kO + sm * DH;
       const int n_own = (n_mine - sm + 1) / 2;  // tiles of this stream
+      auto wait = [&](uint64_t* bar, int parity) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, kDevTimeoutMma));
+        tc_fence_after();
+        return ok;
+      };
+      const uint64_t q_desc = sw128_desc(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc = sw128_desc(smem_u32(sKV), 16, 1024);
+      const uint64_t v_desc = sw128_desc(smem_u32(sKV) + C::kTile, KT * 128, 1024);
+      int k_st = sm;                         // stage of the next scores' tile
+      uint32_t k_ph = 0;
+      auto step = [](int& st, uint32_t& ph) {  // the stream's next tile: two stages on
+        st += 2;
+        if (st >= C::kStages) {
+          st -= C::kStages;
+          ph ^= 1;
+        }
+      };
       // S of the stream's tile n (the CTA's tile 2 n + sm), once its codes are there
       auto scores = [&](int n) -> bool {
-        const int i = 2 * n + sm, st = i % C::kStages;
-        if (!mbar_wait(&kv_full[st], (i / C::kStages) & 1, abort_flag, p.status, kDevTimeoutMma)) return false;
-        tc_fence_after();
-        const uint32_t k_addr = smem_u32(sKV + st * 2 * C::kTile);
+        if (!wait(&kv_full[k_st], k_ph)) return false;
+        const uint64_t kd = k_desc + static_cast<uint32_t>(k_st * 2 * C::kTile) / 16;
+        const uint32_t ts = tbase + (2 * sm + (n & 1)) * KT;
+        if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+          for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int h = 0; h < C::kHalves; ++h)
+            for (int h = 0; h < C::kHalves; ++h)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16_ss(tbase + (2 * sm + (n & 1)) * KT,
-                          sw128_desc(smem_u32(sQ) + (x * C::kHalves + h) * kRows * 128 + k * 32, 16, 1024),
-                          sw128_desc(k_addr + h * KT * 128 + k * 32, 16, 1024), idesc_s,
-                          (x | h | k) != 0 ? 1u : 0u);
-        umma_commit(&s_full[2 * sm + (n & 1)]);
+              for (int k = 0; k < 4; ++k)
+                umma_f16_ss(ts, q_desc + ((x * C::kHalves + h) * kRows * 128 + k * 32) / 16,
+                            kd + (h * KT * 128 + k * 32) / 16, idesc_s, (x | h | k) != 0 ? 1u : 0u);
+          umma_commit(&s_full[2 * sm + (n & 1)]);
+        }
+        __syncwarp();
+        step(k_st, k_ph);
         return true;
       };
       bool ok = (n_own < 1 || scores(0)) && (n_own < 2 || scores(1));
+      int st = sm;
+      uint32_t ph = 0;
       for (int n = 0; ok && n < n_own; ++n) {
-        const int st = (2 * n + sm) % C::kStages, buf = 2 * sm + (n & 1);
-        ok = mbar_wait(&w_full[buf], (n >> 1) & 1, abort_flag, p.status, kDevTimeoutMma);
+        const int buf = 2 * sm + (n & 1);
+        ok = wait(&w_full[buf], (n >> 1) & 1);
         if (!ok) break;
-        tc_fence_after();
-        const uint32_t v_addr = smem_u32(sKV + st * 2 * C::kTile) + C::kTile;
+        const uint64_t vd = v_desc + static_cast<uint32_t>(st * 2 * C::kTile) / 16;
+        const uint32_t tw = tbase + buf * KT;
+        if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
+          for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int k = 0; k < KT / 16; ++k)
-            umma_f16_ts(to, tbase + buf * KT + x * (KT / 2) + k * 8, sw128_desc(v_addr + k * 2048, KT * 128, 1024),
-                        idesc_o, (n | x | k) != 0 ? 1u : 0u);
-        umma_commit(&kv_empty[st]);
-        umma_commit(&o_full[sm]);
-        if (n + 2 < n_own) {
-          // the buffer's next scores replace the weights that this product reads
-          ok = mbar_wait(&o_full[sm], n & 1, abort_flag, p.status, kDevTimeoutMma) && scores(n + 2);
+            for (int k = 0; k < KT / 16; ++k)
+              umma_f16_ts(to, tw + x * (KT / 2) + k * 8, vd + k * 2048 / 16, idesc_o, (n | x | k) != 0 ? 1u : 0u);
+          umma_commit(&kv_empty[st]);
+          umma_commit(&o_full[sm]);
         }
+        __syncwarp();
+        step(st, ph);
+        // the buffer's next scores replace the weights that this product reads
+        if (n + 2 < n_own) ok = wait(&o_full[sm], n & 1) && scores(n + 2);
       }
       griddep_launch_dependents();
     }
