@@ -335,13 +335,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[buf], (n >> 1) & 1, abort_flag, p.status, kDevTimeoutSoftmax));
       if (!ok) break;
       tc_fence_after();
-      uint32_t s[4][16];  // [column half][lane half]
-      auto load = [&]() {
-#pragma unroll
-        for (int h = 0; h < 4; ++h) tmem_ld_16x256b_x4(ts + (h & 1) * kHalf + (h >> 1) * 32, s[h]);
+      // columns 32 q .. + 31 of this warp's rows: s[lane half]
+      auto load = [&](int q, uint32_t (&s)[2][16]) {
+        tmem_ld_16x256b_x4(ts + 32 * q, s[0]);
+        tmem_ld_16x256b_x4(ts + kHalf + 32 * q, s[1]);
         tmem_ld_wait();
       };
-      load();
       uint32_t w[NT][4][8];
       float big[4], lu[4];
       // weights against `ref` (a masked key's scale may be anything)
@@ -354,25 +353,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           nref[y] = f2_pack(-ref[y], -ref[y]);
         }
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          const uint64_t ks = *reinterpret_cast<const uint64_t*>(sc + 8 * g);
-          const uint64_t vs = *reinterpret_cast<const uint64_t*>(sc + KT + 8 * g);
+        for (int q = 0; q < 2; ++q) {
+          uint32_t s[2][16];
+          load(q, s);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int h = (g >> 2) * 2 + (y >> 1), j = 4 * (g & 3) + 2 * (y & 1);
-            float d0, d1, x0, x1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[h][j]), __uint_as_float(s[h][j + 1])), ks, nref[y]), d0, d1);
-            float e0 = fast_exp2(d0), e1 = fast_exp2(d1);
-            f2_unpack(f2_mul(f2_pack(e0, e1), vs), x0, x1);
-            if (mask) {
-              if (k0 + 8 * g >= lim[y]) e0 = x0 = 0.0f;
-              if (k0 + 8 * g + 1 >= lim[y]) e1 = x1 = 0.0f;
+          for (int g = 0; g < 4; ++g) {
+            const int c = 32 * q + 8 * g;
+            const uint64_t ks = *reinterpret_cast<const uint64_t*>(sc + c);
+            const uint64_t vs = *reinterpret_cast<const uint64_t*>(sc + KT + c);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int h = y >> 1, j = 4 * g + 2 * (y & 1);
+              float d0, d1, x0, x1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(s[h][j]), __uint_as_float(s[h][j + 1])), ks, nref[y]), d0, d1);
+              float e0 = fast_exp2(d0), e1 = fast_exp2(d1);
+              f2_unpack(f2_mul(f2_pack(e0, e1), vs), x0, x1);
+              if (mask) {
+                if (k0 + c >= lim[y]) e0 = x0 = 0.0f;
+                if (k0 + c + 1 >= lim[y]) e1 = x1 = 0.0f;
+              }
+              sum[y] = f2_add(sum[y], f2_pack(e0, e1));
+              big[y] = max3f(big[y], fabsf(x0), fabsf(x1));
+              const uint32_t hi = half_pair(x0, x1);
+              w[0][2 * q + h][2 * g + (y & 1)] = hi;
+              if constexpr (kSplit) w[NT - 1][2 * q + h][2 * g + (y & 1)] = half_rest(hi, x0, x1);
             }
-            sum[y] = f2_add(sum[y], f2_pack(e0, e1));
-            big[y] = max3f(big[y], fabsf(x0), fabsf(x1));
-            const uint32_t hi = half_pair(x0, x1);
-            w[0][h][2 * (g & 3) + (y & 1)] = hi;
-            if constexpr (kSplit) w[NT - 1][h][2 * (g & 3) + (y & 1)] = half_rest(hi, x0, x1);
           }
         }
 #pragma unroll
@@ -406,7 +411,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             search = search || (big[y] >= kMaxWeight && !(tries == 0 && big[y] < 1e30f));
           }
           search = __any_sync(0xffffffffu, search);
-          load();
         } else {
 #pragma unroll
           for (int y = 0; y < 4; ++y) big[y] = INFINITY;
@@ -417,18 +421,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int y = 0; y < 4; ++y) top[y] = top_w[y] = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < 8; ++g)
+          for (int q = 0; q < 2; ++q) {
+            uint32_t s[2][16];
+            load(q, s);
 #pragma unroll
-            for (int z = 0; z < 2; ++z) {
-              const float ks = sc[8 * g + z], lv = weight_log2(0.0f, sc[KT + 8 * g + z]);
+            for (int g = 0; g < 4; ++g)
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const float v = __uint_as_float(s[(g >> 2) * 2 + (y >> 1)][4 * (g & 3) + 2 * (y & 1) + z]);
-                const float x = k0 + 8 * g + z < lim[y] ? v * ks : -INFINITY;
-                top[y] = fmaxf(top[y], x);
-                top_w[y] = fmaxf(top_w[y], x + lv);
+              for (int z = 0; z < 2; ++z) {
+                const int c = 32 * q + 8 * g + z;
+                const float ks = sc[c], lv = weight_log2(0.0f, sc[KT + c]);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const float v = __uint_as_float(s[y >> 1][4 * g + 2 * (y & 1) + z]);
+                  const float x = k0 + c < lim[y] ? v * ks : -INFINITY;
+                  top[y] = fmaxf(top[y], x);
+                  top_w[y] = fmaxf(top_w[y], x + lv);
+                }
               }
-            }
+          }
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
 #pragma unroll
