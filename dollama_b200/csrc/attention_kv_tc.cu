@@ -29,10 +29,6 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kTcThreads = 512;  // 4 warpgroups: softmax A, softmax B, MMA issuers, conversion
-// Registers a thread of each warpgroup (launched with 128 each): what the issuers and the conversion
-// give back goes to the softmax, whose scores and weights of a tile stay in registers.
-constexpr int kRegsSoftmax = 168, kRegsIssue = 64, kRegsConvert = 112;
-static_assert(2 * kRegsSoftmax + kRegsIssue + kRegsConvert <= 4 * 128, "the register split");
 constexpr int kConvThreads = 128;
 
 constexpr int KT = 64;  // keys per tile
@@ -164,13 +160,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tbase = *tmem_slot;
 
-  // Every warp meets here once it has its registers: a warpgroup that is done at once (no keys) must not
-  // take back what the softmax is still waiting for.
-  auto split_done = [] { asm volatile("bar.sync 1, 512;" ::: "memory"); };
   if (warp >= 12) {
     // ================================================================ codes -> fp16
-    regs_dec<kRegsConvert>();
-    split_done();
     const int t = threadIdx.x - 384;
     constexpr int kPieces = DH / 16;                    // 16-code pieces of a row
     constexpr int kEach = KT * kPieces / kConvThreads;  // pieces a thread converts, of K and of V
@@ -230,12 +221,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         ph ^= 1;
       }
     }
-    __syncwarp();
-    regs_inc<128>();
   } else if (warp >= 8) {
     // ================================================================ MMA issuer of one stream
-    regs_dec<kRegsIssue>();
-    split_done();
     const int sm = __shfl_sync(0xffffffffu, warp, 0) - 8;
     if (sm < 2) {
       constexpr uint32_t idesc_s = idesc_f16_f32(kRows, KT, false);
@@ -304,12 +291,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       griddep_launch_dependents();
     }
-    __syncwarp();
-    regs_inc<128>();
   } else {
     // ================================================================ softmax of one stream
-    regs_inc<kRegsSoftmax>();
-    split_done();
     const int sm = warp >> 2, gr = lane >> 2, c4 = lane & 3;
     const int row0 = (warp & 3) * 32 + gr;  // this lane's rows: row0 + 8 y
     constexpr uint32_t kHalf = 16u << 16;   // TMEM address of 16 lanes further
@@ -504,8 +487,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         s_l[sm * kRows + row0 + 8 * y] = l[y];
       }
     }
-    __syncwarp();
-    regs_dec<128>();  // what follows runs with an even split again
   }
   __syncthreads();  // every product is done: Q and the ring are free
 

@@ -502,19 +502,6 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, uint32_t cta)
       : "memory");
 }
 
-// ---------------------------------------------------------------- register split
-// Gives registers of this warpgroup back (dec) or takes some of those given back (inc); kRegs is the
-// thread's new count, a multiple of 8.  Over all warpgroups the new counts must not add up to more than
-// the block was launched with, and every warp of the group executes it.
-template <int kRegs>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-template <int kRegs>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-
 // ---------------------------------------------------------------- descriptors
 // Shared-memory matrix descriptor for a 128-byte-swizzled operand tile whose rows are
 // 128 bytes (64 fp16) and whose 8-row swizzle atoms are 1024 bytes apart.  For a K-major
