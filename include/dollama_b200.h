@@ -331,12 +331,14 @@ int dlm_bitnet_weight_info(const dlm_bitnet_config* cfg, int index, char* name, 
  *   dlm_add_rms_norm_i8 -> dlm_gemm_i8 (q|k|v) -> dlm_kv_i8_append -> dlm_attention_kv_i8 ->
  *   dlm_quantize_act_i8 -> dlm_gemm_i8 (out) -> dlm_add_rms_norm_i8 -> ...
  * The reference has no counterpart (its LM is ternary with an fp32 cache).  `dtype` is a dlm_dtype.
- * Row strides (ld*) are in elements.  int8 codes follow dlm_quantize_act_i8: with a = max|x| over
- * the row, scale = a / 127 and code = round(127 x / a), halves away from zero; an all-zero row has
- * scale 0 and codes 0; a row with a NaN or an infinity has scale NaN and codes 0, so that whatever
- * is computed from it is NaN.  Weights are quantized per channel by dlm_quantize_act_i8 on [N, K].
+ * Row strides (ld*) are in elements.  int8 codes follow the rule of dlm_quantize_act_i8: with a =
+ * max|x| over the row, scale = a / 127 and code = round(127 x / a), halves away from zero; an
+ * all-zero row has scale 0 and codes 0.  In this section a row with a NaN or an infinity has scale
+ * NaN and codes 0, so that whatever is computed from it is NaN.  Weights are quantized per channel
+ * by dlm_quantize_act_i8 on their fp32 [N, K].
  * No call allocates, synchronises or keeps state: all may be captured into CUDA graphs, and calls
- * on different streams may overlap as long as their outputs are distinct.
+ * on different streams may overlap as long as their outputs are distinct.  Pointers and stream
+ * belong to the current device.
  */
 
 /* RMS norm with the residual's addition, and an int8 output:
@@ -383,8 +385,8 @@ int dlm_kv_i8_read(const int8_t* kq, const float* kscale, const int8_t* vq, cons
  * [0, kv_len[b] - q_len[b] + i]; with causal == 0 every query sees keys [0, kv_len[b]).  A query
  * that sees no key gets zeros; queries from q_len[b] on are not written; keys that a query does not
  * see do not touch its result, whatever they hold.  A kv_len outside [0, Lmax] is clamped and
- * raises the device status word (code 6).  kv_len, q_len: device int32 [B].  Dh 64 or 128; q and out
- * rows on 16-byte boundaries.  Softmax statistics and sums are fp32; fp32 inputs keep 22 bits or
+ * raises the device status word (code 6); a q_len above Sq counts as Sq, below 0 as 0.  kv_len,
+ * q_len: device int32 [B].  Dh 64 or 128; Lmax <= 2^30; q and out rows on 16-byte boundaries.  Softmax statistics and sums are fp32; fp32 inputs keep 22 bits or
  * more of q and of the weights, 16-bit inputs 11 of the weights. */
 int dlm_attention_kv_i8(const void* q, int ldq, const int8_t* kq, const float* kscale,
                         const int8_t* vq, const float* vscale, void* out, int ldo, int B, int Hq,

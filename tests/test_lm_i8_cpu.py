@@ -65,7 +65,8 @@ CASES = [
     (attn, dict(Hkv=0), INVALID), (attn, dict(ldq=255), INVALID), (attn, dict(ldo=252, Hq=4), INVALID),
     (attn, dict(Dh=80), UNSUPPORTED), (attn, dict(scale=float("nan")), INVALID),
     (attn, dict(scale=float("inf")), INVALID), (attn, dict(q=A + 4), INVALID), (attn, dict(t=1, ldq=260), INVALID),
-    (attn, dict(B=-1), INVALID), (attn, dict(t=9), INVALID),
+    (attn, dict(B=-1), INVALID), (attn, dict(t=9), INVALID), (attn, dict(Lm=(1 << 30) + 1), UNSUPPORTED),
+    (attn, dict(Sq=1 << 30), UNSUPPORTED),
 ]
 
 

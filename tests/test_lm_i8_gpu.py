@@ -173,7 +173,7 @@ def check_gemm(xq, xs, wq, ws, b, y, t, M, N, K):
                                    (32, 4096, 4096), (33, 257, 1040), (64, 512, 1536), (65, 640, 640), (100, 96, 48),
                                    (128, 128, 128), (129, 127, 272), (200, 5, 4096), (256, 512, 512),
                                    (1003, 2111, 1360), (300, 16000, 512), (2048, 1536, 512), (1, 16000, 512),
-                                   (2050, 4100, 2064), (3, 40, 16384)])
+                                   (2050, 4100, 2064), (3, 40, 16384), (3000, 2111, 272)])
 @pytest.mark.parametrize("bias", [False, True])
 def test_gemm(t, M, N, K, bias):
     a = make_gemm(M, N, K, t, bias)
@@ -453,6 +453,47 @@ def test_attention_strides(t):
     assert (wide[..., Hq * Dh:] == -3).all()
 
 
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("g,Dh", [(1, 64), (4, 128), (12, 64)])
+def test_attention_many_sequences(t, g, Dh):
+    """More (sequence, kv head) pairs than the SMs hold CTAs: one warp for each, ragged lengths."""
+    B, Hkv, Lm = 900, 3, 70
+    gn, ty = gen(g), O.TYPES[t]
+    q = torch.randn(B, 1, Hkv * g, Dh, generator=gn, device="cuda").to(ty)
+    cache = make_cache(B, Hkv, Lm, Dh, gn)
+    kv = torch.randint(0, Lm + 1, (B,), generator=gn, device="cuda", dtype=torch.int32)
+    out = run_attn(q, cache, kv, None, True, t)
+    pick = torch.arange(0, B, 47, device="cuda")
+    check_attn(q[pick], [c[pick] for c in cache], kv[pick], None, True, t, out[pick])
+    # a sequence's result does not depend on the batch around it beyond the order of its sums
+    one = run_attn(q[3:4].contiguous(), [c[3:4].contiguous() for c in cache], kv[3:4], None, True, t)
+    check_attn(q[3:4], [c[3:4] for c in cache], kv[3:4], None, True, t, one)
+
+
+@pytest.mark.parametrize("Sq,Hq,Hkv", [(127, 1, 1), (129, 1, 1), (43, 6, 2), (300, 5, 1), (17, 16, 16)])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_attention_row_tiles(t, Sq, Hq, Hkv):
+    """Rows that end inside a tile, groups of heads that no tile divides, keys split over clusters."""
+    g, ty = gen(Sq), O.TYPES[t]
+    q = torch.randn(1, Sq, Hq, 128, generator=g, device="cuda").to(ty)
+    cache = make_cache(1, Hkv, 700, 128, g)
+    kv = torch.tensor([691], dtype=torch.int32, device="cuda")
+    out = run_attn(q, cache, kv, None, True, t)
+    pick = [0, 1, Sq // 2, Sq - 2, Sq - 1]
+    for i in pick:  # query i alone is the last of a shorter sequence
+        n = torch.tensor([691 - Sq + i + 1], dtype=torch.int32, device="cuda")
+        check_attn(q[:, i:i + 1].contiguous(), cache, n, None, True, t, out[:, i:i + 1])
+
+
+def test_attention_without_a_cache_is_zero():
+    q = torch.randn(2, 3, 4, 64, device="cuda")
+    out = torch.full_like(q, 5.0)
+    kv = torch.zeros(2, dtype=torch.int32, device="cuda")
+    L.call("dlm_attention_kv_i8", _p(q), 256, None, None, None, None, _p(out), 256, 2, 4, 2, 3, 64, 0, _p(kv), None, 1,
+           0.125, F32, _s())
+    assert (out == 0).all()
+
+
 def test_attention_length_outside_is_clamped_and_reported():
     g = gen(6)
     q = torch.randn(2, 1, 2, 64, generator=g, device="cuda")
@@ -500,6 +541,82 @@ def test_repeated_calls_are_bit_identical():
         assert torch.equal(first, run_attn(q, cache, kv, None, True, F32))
         run_gemm(*a, F16, 16, 512, 2048)
         assert torch.equal(y0, a[5])
+
+
+def test_calls_on_two_streams_at_once():
+    """The same operators on two streams, in turn, each with its own outputs."""
+    work = []
+    for k in range(2):
+        g = gen(50 + k)
+        q = torch.randn(4, 30, 4, 64, generator=g, device="cuda").half()
+        cache = make_cache(4, 2, 900, 64, g)
+        kv = torch.full((4,), 880, dtype=torch.int32, device="cuda")
+        work.append((q, cache, kv, make_gemm(300, 700, 1040, F16, True, seed=k)))
+    want = []
+    for q, cache, kv, a in work:
+        run_gemm(*a, F16, 300, 700, 1040)
+        want.append((run_attn(q, cache, kv, None, True, F16), a[5].clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    outs = [torch.zeros_like(w[0]) for w in work]
+    for _ in range(10):
+        for s, o, (q, cache, kv, a) in zip(streams, outs, work):
+            with torch.cuda.stream(s):
+                run_gemm(*a, F16, 300, 700, 1040)
+                run_attn(q, cache, kv, None, True, F16, out=o)
+    torch.cuda.synchronize()
+    for (o, (w, y), (_, _, _, a)) in zip(outs, want, work):
+        assert torch.equal(o, w) and torch.equal(a[5], y)
+
+
+_FIRST = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from tests import test_lm_i8_gpu as G
+torch.zeros(1, device="cuda")
+g = torch.Generator(device="cuda").manual_seed(1)
+x = torch.randn(40, 256, generator=g, device="cuda").half()
+w = torch.ones(256, device="cuda").half()
+h, q, s = torch.empty_like(x), torch.empty(40, 256, dtype=torch.int8, device="cuda"), torch.empty(40, device="cuda")
+wq = torch.randint(-127, 128, (256, 256), device="cuda", dtype=torch.int8)
+ws = torch.rand(256, device="cuda")
+y = torch.empty(40, 256, device="cuda").half()
+cache = [torch.zeros(2, 2, 64, 64, dtype=torch.int8, device="cuda"), torch.zeros(2, 2, 64, device="cuda")]
+cache += [c.clone() for c in cache]
+pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+kv = torch.full((2,), 20, dtype=torch.int32, device="cuda")
+qq = torch.randn(2, 20, 4, 64, device="cuda").half()
+o, one = torch.empty_like(qq), torch.empty(2, 1, 4, 64, device="cuda").half()
+def all_of_them():
+    G.L.call("dlm_add_rms_norm_i8", x.data_ptr(), 256, None, 0, w.data_ptr(), h.data_ptr(), 256, q.data_ptr(),
+             s.data_ptr(), 40, 256, 1e-5, 1, G._s())
+    G.run_gemm(q, s, wq, ws, None, y, 1, 40, 256, 256)
+    G.L.call("dlm_kv_i8_append", y.data_ptr(), 256, y.data_ptr() + 256, 256, *[c.data_ptr() for c in cache], 2, 20, 2, 64,
+             64, pos.data_ptr(), None, 1, G._s())
+    G.run_attn(qq, cache, kv, None, True, 1, out=o)
+    G.run_attn(qq[:, :1].contiguous(), cache, kv, None, True, 1, out=one)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    all_of_them()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in (q, s, y, *cache, o)]
+all_of_them()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, (q, s, y, *cache, o)))
+print("captured first")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first call of each operator is captured (no warm-up)."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parent.parent)
+    r = subprocess.run([sys.executable, "-c", _FIRST, root], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
 
 
 # ------------------------------------------------------------------ together
