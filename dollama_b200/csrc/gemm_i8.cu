@@ -5,12 +5,20 @@
 // on tcgen05.mma kind::i8.  The sum is exact (int32 accumulators in tensor memory, |sum| <= 128^2 K
 // < 2^31); the epilogue is fp32 with one rounding to T.
 //
-// Two kernels:
+// Two kernels, chosen by estimated time (launch_best):
 //   gemm_i8_kernel     persistent, tiles of tokens x channels, double-buffered accumulators: a CTA
-//                      pair (cta_group::2) per 256 x 256 tile, or a CTA per 128 x 128 tile;
-//   gemm_i8_k_kernel   for few tiles: 128 channels (the MMA's M operand) x up to 128 tokens per
+//                      pair (cta_group::2) per 256 x 256 tile, or a CTA per 128 x 128 tile.  Bound by
+//                      the tensor cores and the power limit for large K (8192 x 8192 x 4096, fp16 out:
+//                      177 us, 3100 TOP/s; with one CTA per 128 x 128 tile 329 us, bound by operand
+//                      reads from L2: 128 bytes a clock and SM asked for, about 64 served), by the
+//                      epilogue's conversions and the output's bytes for small K (4096 x 16000 x 512:
+//                      48 us for 137 MB);
+//   gemm_i8_k_kernel   for few tokens: 128 channels (the MMA's M operand) x up to 128 tokens per
 //                      cluster, whose CTAs split K and add their integer partial sums over
-//                      distributed shared memory (integers: any order gives the same sum).
+//                      distributed shared memory (integers: any order gives the same sum).  Bound by
+//                      the weight's bytes and by latency (32 x 4096 x 4096: 6.5 us, the weight's bytes
+//                      alone 2.6).
+#include <cmath>
 #include <cstdint>
 
 #include "dtype.cuh"
@@ -69,9 +77,8 @@ __device__ __forceinline__ void tile_at(const GemmI8Params& p, int t, int& mt, i
   mt = g * kGroup + (r - nt * rows);
 }
 
-// wscale (and bias) of 32 consecutive channels, the same for every lane; zero beyond N
-template <typename T>
-__device__ __forceinline__ void channel_terms(const GemmI8Params& p, int n, float (&w)[32], float (&b)[32]) {
+// wscale of 32 consecutive channels, the same for every lane; zero beyond N
+__device__ __forceinline__ void channel_scales(const GemmI8Params& p, int n, float (&w)[32]) {
   if (p.ws_vec && n + 32 <= p.N) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -85,48 +92,56 @@ __device__ __forceinline__ void channel_terms(const GemmI8Params& p, int n, floa
 #pragma unroll
     for (int j = 0; j < 32; ++j) w[j] = n + j < p.N ? __ldg(p.ws + n + j) : 0.0f;
   }
-  const T* bias = static_cast<const T*>(p.bias);
-#pragma unroll
-  for (int j = 0; j < 32; ++j) b[j] = bias && n + j < p.N ? to_f(bias[n + j]) : 0.0f;
 }
 
 // This warp's 32 rows x `cols` channels of an accumulator (TMEM address ta) to y, 128 bytes of each
 // row at a time through its staging buffer (16-byte pieces XORed with the row: no bank conflicts, and
-// the layout that the 128-byte-swizzled tensor store reads).
+// the layout that the 128-byte-swizzled tensor store reads).  A chunk is finished in registers before
+// it waits for the buffer, so the previous chunk's store runs under it.
 template <typename T>
 __device__ __forceinline__ void epilogue(const GemmI8Params& p, const CUtensorMap* tmY, uint32_t ta, int row0,
                                          int n0, int cols, uint8_t* stage) {
   constexpr int kCols = 128 / static_cast<int>(sizeof(T));  // columns of a staged row
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));
   const int lane = threadIdx.x & 31;
   const float xs = row0 + lane < p.M ? p.xs[row0 + lane] : 0.0f;
   T* y = static_cast<T*>(p.y);
+  const T* bias = static_cast<const T*>(p.bias);
   for (int c0 = 0; c0 < cols && n0 + c0 < p.N; c0 += kCols) {
+    uint4 o[8];
+#pragma unroll
+    for (int h = 0; h < kCols; h += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(ta + c0 + h, r);
+      float w[32];
+      const int n = n0 + c0 + h;
+      channel_scales(p, n, w);
+      tmem_ld_wait();
+      float v[32];
+      if (bias) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          v[j] = fmaf(static_cast<float>(static_cast<int>(r[j])) * xs, w[j], n + j < p.N ? to_f(bias[n + j]) : 0.0f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = static_cast<float>(static_cast<int>(r[j])) * xs * w[j];
+      }
+#pragma unroll
+      for (int q = 0; q < 32 / kPer; ++q) {
+        Vec<T, kPer> t;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) t.v[j] = from_f<T>(v[q * kPer + j]);
+        o[h / kPer + q] = *reinterpret_cast<const uint4*>(&t);
+      }
+    }
     if (p.y_tma) {  // the previous store has read the buffer
       if (lane == 0) bulk_wait_read_le0();
       __syncwarp();
     }
 #pragma unroll
-    for (int h = 0; h < kCols; h += 32) {
-      uint32_t r[32];
-      tmem_ld_32x32b_x32(ta + c0 + h, r);
-      float w[32], b[32];
-      channel_terms<T>(p, n0 + c0 + h, w, b);
-      tmem_ld_wait();
-#pragma unroll
-      for (int q = 0; q < 2 * static_cast<int>(sizeof(T)); ++q) {
-        constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-        Vec<T, kPer> o;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-          const int i = q * kPer + j;
-          o.v[j] = from_f<T>(fmaf(static_cast<float>(static_cast<int>(r[i])) * xs, w[i], b[i]));
-        }
-        const int piece = h * static_cast<int>(sizeof(T)) / 16 + q;
-        *reinterpret_cast<Vec<T, kPer>*>(stage + lane * 128 + ((piece ^ (lane & 7)) << 4)) = o;
-      }
-    }
+    for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(stage + lane * 128 + ((q ^ (lane & 7)) << 4)) = o[q];
     // a bulk-tensor store writes whole 16-byte pieces: an odd last piece goes element by element
-    if (p.y_tma && (n0 + c0 + kCols <= p.N || p.N % (16 / static_cast<int>(sizeof(T))) == 0)) {
+    if (p.y_tma && (n0 + c0 + kCols <= p.N || p.N % kPer == 0)) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -474,39 +489,55 @@ __global__ void __launch_bounds__(kKThreads)
   else
     __syncthreads();
   if (*abort_flag == 0) {
-    // this CTA's share of the tile, four channels at a time
+    // this CTA's share of the tile's tokens; a thread keeps four channels (their scales are read once,
+    // read for every token they took three times the whole product at 128 tokens x 512)
+    constexpr int kQuads = kBM / 4, kRowsPer = kKThreads / kQuads;
     const int rows = min(NT, p.M - m0);
-    const int quads = rows * (kBM / 4);
-    const int q0 = quads * rank / p.C, q1 = quads * (rank + 1) / p.C;
+    const int m1 = rows * (rank + 1) / p.C;
+    const int qd = threadIdx.x % kQuads, n = n0 + 4 * qd;
     T* y = static_cast<T*>(p.y);
     const T* bias = static_cast<const T*>(p.bias);
-    for (int q = q0 + threadIdx.x; q < q1; q += kKThreads) {
-      const int m = m0 + q / (kBM / 4), n = n0 + 4 * (q % (kBM / 4));
-      if (n >= p.N) continue;
-      const uint32_t addr = smem_u32(smem) + 16 * q;
-      int s[4] = {0, 0, 0, 0};
-      for (int c = 0; c < p.C; ++c) {
-        const uint4 v = p.C > 1 ? ld_dsmem16(addr, c) : reinterpret_cast<const uint4*>(smem)[q];
-        s[0] += static_cast<int>(v.x);
-        s[1] += static_cast<int>(v.y);
-        s[2] += static_cast<int>(v.z);
-        s[3] += static_cast<int>(v.w);
-      }
-      const float xs = p.xs[m];
-      T* dst = y + static_cast<size_t>(m) * p.ldy + n;
-      Vec<T, 4> o;
+    float w[4], b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = n + j < p.N;
-        const float b = bias && in ? to_f(bias[n + j]) : 0.0f;
-        o.v[j] = from_f<T>(fmaf(static_cast<float>(s[j]) * xs, in ? p.ws[n + j] : 0.0f, b));
-      }
-      if (p.y_tma && n + 4 <= p.N) {
-        *reinterpret_cast<Vec<T, 4>*>(dst) = o;
-      } else {
+    for (int j = 0; j < 4; ++j) {
+      w[j] = n + j < p.N ? p.ws[n + j] : 0.0f;
+      b[j] = bias && n + j < p.N ? to_f(bias[n + j]) : 0.0f;
+    }
+    if (n < p.N) {
+#pragma unroll 4
+      for (int m = rows * rank / p.C + threadIdx.x / kQuads; m < m1; m += kRowsPer) {
+        const int q = m * kQuads + qd;
+        const uint32_t addr = smem_u32(smem) + 16 * q;
+        const float xs = p.xs[m0 + m];
+        int s[4] = {0, 0, 0, 0};
+        if (p.C == 1) {
+          const uint4 v = reinterpret_cast<const uint4*>(smem)[q];
+          s[0] = static_cast<int>(v.x);
+          s[1] = static_cast<int>(v.y);
+          s[2] = static_cast<int>(v.z);
+          s[3] = static_cast<int>(v.w);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) dst[j] = o.v[j];
+          for (int c = 0; c < 8; ++c)
+            if (c < p.C) {
+              const uint4 v = ld_dsmem16(addr, c);
+              s[0] += static_cast<int>(v.x);
+              s[1] += static_cast<int>(v.y);
+              s[2] += static_cast<int>(v.z);
+              s[3] += static_cast<int>(v.w);
+            }
+        }
+        T* dst = y + static_cast<size_t>(m0 + m) * p.ldy + n;
+        Vec<T, 4> o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.v[j] = from_f<T>(fmaf(static_cast<float>(s[j]) * xs, w[j], b[j]));
+        if (p.y_tma && n + 4 <= p.N) {
+          *reinterpret_cast<Vec<T, 4>*>(dst) = o;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.N) dst[j] = o.v[j];
+        }
       }
     }
   }
@@ -597,25 +628,97 @@ int launch(const int8_t* xq, long long ldx, const int8_t* w, GemmI8Params p, cud
   return DLM_OK;
 }
 
+// Clusters of C CTAs that run at once (they have to fit inside the groups of SMs that share a cluster,
+// so this is less than the SMs divided by C).
 template <int NT, typename T>
-int launch_k(const int8_t* xq, long long ldx, const int8_t* w, GemmI8Params p, cudaStream_t s) {
-  using C = KCfg<NT>;
-  static bool done[64] = {false};
-  const int rc = allow_smem(gemm_i8_k_kernel<NT, T>, C::kSmem, done);
-  if (rc != DLM_OK) return rc;
+int resident_clusters(int C) {
+  static int cache[64][4] = {{0}};
+  int dev = 0;
+  const int i = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return num_sms() / C;
+  if (cache[dev][i] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(C);
+    cfg.blockDim = dim3(kKThreads);
+    cfg.dynamicSmemBytes = KCfg<NT>::kSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = C;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_k_kernel<NT, T>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = num_sms() / C > 0 ? num_sms() / C : 1;
+    }
+    cache[dev][i] = n;
+  }
+  return cache[dev][i];
+}
+
+// Estimated microseconds of a launch, fitted to measured times of 91 shapes (M 1..4096, N and K
+// 512..16000): fixed part plus waves of tiles times their k-blocks.  Where two kernels are within a few
+// percent either may be taken.
+struct Estimate {
+  double us;
+  int C;  // of gemm_i8_k_kernel
+};
+
+double tiles_of(int M, int N, int bm, int bn) {
+  return static_cast<double>((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+}
+
+// 128 x 128 tiles, one per SM: 512 x 512 x 512 5.1 us, 1024 x 8192 x 4096 35.8 us
+double estimate_single(int M, int N, int nkb) {
+  return 3.6 + std::ceil(tiles_of(M, N, 128, 128) / num_sms()) * (0.9 + 0.225 * nkb);
+}
+// 256 x 256 tiles, one per pair: 512 x 512 x 512 7.3 us, 1024 x 8192 x 4096 27.2 us
+double estimate_pair(int M, int N, int nkb) {
+  return 5.5 + std::ceil(tiles_of(M, N, 256, 256) / (num_sms() / 2)) * (2.8 + 0.29 * nkb);
+}
+// K split over clusters; up to NT tokens: 32 x 4096 x 4096 6.7 us (128 x 128 tiles: 10.8 us)
+template <int NT, typename T>
+Estimate estimate_k(int M, int N, int nkb) {
+  constexpr double kFixed = NT == 16 ? 3.4 : NT == 32 ? 4.4 : NT == 64 ? 5.9 : 8.0;
+  constexpr double kBlock = NT == 16 ? 0.127 : NT == 32 ? 0.14 : NT == 64 ? 0.17 : 0.225;
+  Estimate best{1e30, 1};
+  for (int C = 1; C <= 8 && (C == 1 || nkb >= 2 * C); C *= 2) {
+    const double waves = std::ceil(tiles_of(M, N, NT, 128) / resident_clusters<NT, T>(C));
+    const double us = 2.0 + (C > 1 ? 0.3 : 0.0) + waves * (kFixed - 2.0 + ((nkb + C - 1) / C) * kBlock);
+    if (us < best.us) best = Estimate{us, C};
+  }
+  return best;
+}
+
+template <int NT, typename T>
+int launch_k(const int8_t* xq, long long ldx, const int8_t* w, GemmI8Params p, int C, cudaStream_t s) {
+  using K = KCfg<NT>;
   CUtensorMap tx, tw;
   if (!tmap_i8(&tx, xq, p.M, p.K, ldx, NT) || !tmap_i8(&tw, w, p.N, p.K, p.K, kBM)) return DLM_ERR_CUDA;
   p.m_tiles = (p.M + NT - 1) / NT;
   p.n_tiles = (p.N + kBM - 1) / kBM;
-  const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles;
-  DLM_REQUIRE(tiles < (1ll << 27), DLM_ERR_UNSUPPORTED, "gemm_i8: too many tiles");
-  // the SMs filled about once, two k-blocks at least for each CTA
-  const int nkb = (p.K + kKB - 1) / kKB;
-  p.C = 1;
-  while (p.C < 8 && 2 * p.C * tiles <= num_sms() && nkb >= 4 * p.C) p.C *= 2;
-  DLM_CHECK_CUDA(launch_cluster(gemm_i8_k_kernel<NT, T>, static_cast<int>(tiles) * p.C, kKThreads, C::kSmem, p.C,
-                                s, tx, tw, p));
+  p.C = C;
+  const long long ctas = static_cast<long long>(p.m_tiles) * p.n_tiles * C;
+  DLM_REQUIRE(ctas < (1ll << 30), DLM_ERR_UNSUPPORTED, "gemm_i8: too many tiles");
+  DLM_CHECK_CUDA(launch_cluster(gemm_i8_k_kernel<NT, T>, static_cast<int>(ctas), kKThreads, K::kSmem, C, s, tx, tw,
+                                p));
   return DLM_OK;
+}
+
+// The kernel of least estimated time.
+template <int NT, typename T>
+int launch_best(const int8_t* xq, long long ldx, const int8_t* w, const GemmI8Params& p, cudaStream_t s) {
+  static bool done[64] = {false};
+  const int rc = allow_smem(gemm_i8_k_kernel<NT, T>, KCfg<NT>::kSmem, done);
+  if (rc != DLM_OK) return rc;
+  const int nkb = (p.K + kKB - 1) / kKB;
+  const double single = estimate_single(p.M, p.N, nkb), pair = estimate_pair(p.M, p.N, nkb);
+  const Estimate split = estimate_k<NT, T>(p.M, p.N, nkb);
+  if (split.us <= single && split.us <= pair) return launch_k<NT, T>(xq, ldx, w, p, split.C, s);
+  if (pair < single) return launch<true, T>(xq, ldx, w, p, s);
+  return launch<false, T>(xq, ldx, w, p, s);
 }
 
 }  // namespace
@@ -642,19 +745,10 @@ extern "C" int dlm_gemm_i8(const int8_t* xq, int ldx, const float* xscale, const
   GemmI8Params p{xscale, wscale, bias, y, ldy, M, N, K, 0, 0, 1,
                  aligned16(y) && ldy % static_cast<int>(16 / e) == 0, aligned16(wscale), device_status_ptr()};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  auto tiles = [&](long long bm, long long bn) { return (M + bm - 1) / bm * ((N + bn - 1) / bn); };
-  // few tokens, or too few 128 x 128 tiles for the SMs: K split over clusters; else the CTA pairs once
-  // their 256 x 256 tiles fill most of the SMs
-  const bool split = M <= 64 || 2 * tiles(128, 128) <= num_sms();
-  const bool pair = tiles(256, 256) >= num_sms() / 2;
   DLM_DISPATCH_DTYPE(dtype, T, {
-    if (split) {
-      if (M <= 16) return launch_k<16, T>(xq, ldx, w, p, s);
-      if (M <= 32) return launch_k<32, T>(xq, ldx, w, p, s);
-      if (M <= 64) return launch_k<64, T>(xq, ldx, w, p, s);
-      return launch_k<128, T>(xq, ldx, w, p, s);
-    }
-    if (pair) return launch<true, T>(xq, ldx, w, p, s);
-    return launch<false, T>(xq, ldx, w, p, s);
+    if (M <= 16) return launch_best<16, T>(xq, ldx, w, p, s);
+    if (M <= 32) return launch_best<32, T>(xq, ldx, w, p, s);
+    if (M <= 64) return launch_best<64, T>(xq, ldx, w, p, s);
+    return launch_best<128, T>(xq, ldx, w, p, s);
   });
 }

@@ -6,6 +6,10 @@
     python -m dollama_b200.kernel_bench gn --n 1 --h 512 --w 512 --cin 512
     python -m dollama_b200.kernel_bench vae --h 128 --w 128            # whole decode (graph)
     python -m dollama_b200.kernel_bench lm --b 256 --sq 64 --sk 128    # prefill 64 + greedy to 128
+    python -m dollama_b200.kernel_bench norm_i8 --m 16384 --k 4096     # add + RMS norm + int8
+    python -m dollama_b200.kernel_bench gemm_i8 --m 32 --n 4096 --k 4096
+    python -m dollama_b200.kernel_bench kv_i8 --b 16 --sq 2048 --heads 8 --dh 128   # write + read
+    python -m dollama_b200.kernel_bench attn_i8 --b 8 --sq 1 --heads 32 --kv-heads 8 --sk 16384 --dh 128
 
 Prints one JSON line: shape, microseconds per launch, achieved TFLOP/s and the fraction of the
 measured bf16 peak (MEASURED_PEAKS.json next to the repository, when present).  Used for the
@@ -64,9 +68,58 @@ def _time(fn, iters, warm=3):
     return e0.elapsed_time(e1) / iters
 
 
+def _int8_op(a, dev):
+    """The int8 language-model operators: the call, its operations and its shape (bytes: each input
+    read once, each output written once)."""
+    t, ty, e = {"f32": (L.F32, torch.float32, 4), "f16": (L.F16, torch.float16, 2),
+                "bf16": (L.BF16, torch.bfloat16, 2)}[a.dtype]
+    codes = lambda *s: torch.randint(-127, 128, s, dtype=torch.int8, device=dev)
+    if a.op == "norm_i8":
+        x, r = (torch.randn(a.m, a.k, device=dev).to(ty) for _ in range(2))
+        w, h = torch.ones(a.k, device=dev).to(ty), torch.empty_like(x)
+        q, s = torch.empty(a.m, a.k, dtype=torch.int8, device=dev), torch.empty(a.m, device=dev)
+        fn = lambda: L.call("dlm_add_rms_norm_i8", _p(x), a.k, _p(r), a.k, _p(w), _p(h), a.k, _p(q), _p(s),
+                            a.m, a.k, 1e-5, t, _s())
+        return fn, 0.0, {"m": a.m, "k": a.k, "bytes": a.m * a.k * (3.0 * e + 1)}
+    if a.op == "gemm_i8":
+        x, w = codes(a.m, a.k), codes(a.n, a.k)
+        xs, ws = torch.rand(a.m, device=dev), torch.rand(a.n, device=dev)
+        y = torch.empty(a.m, a.n, device=dev, dtype=ty)
+        fn = lambda: L.call("dlm_gemm_i8", _p(x), a.k, _p(xs), _p(w), _p(ws), None, _p(y), a.n, a.m, a.n, a.k, t,
+                            _s())
+        return fn, 2.0 * a.m * a.n * a.k, {"m": a.m, "n": a.n, "k": a.k,
+                                           "bytes": a.m * a.k + a.n * a.k + e * a.m * a.n}
+    H = a.kv_heads or a.heads
+    Lm = a.sq if a.op == "kv_i8" else a.sk
+    cache = [codes(a.b, H, Lm, a.dh), torch.rand(a.b, H, Lm, device=dev) / 64]
+    cache += [c.clone() for c in cache]
+    c = [_p(x) for x in cache]
+    if a.op == "kv_i8":
+        k, v = (torch.randn(a.b, a.sq, H * a.dh, device=dev).to(ty) for _ in range(2))
+        pos = torch.zeros(a.b, dtype=torch.int32, device=dev)
+
+        def fn():
+            W = H * a.dh
+            shape = (a.b, a.sq, H, a.dh, Lm, _p(pos), None, t, _s())
+            L.call("dlm_kv_i8_append", _p(k), W, _p(v), W, *c, *shape)
+            L.call("dlm_kv_i8_read", *c, _p(k), W, _p(v), W, *shape)
+        return fn, 0.0, {"b": a.b, "s": a.sq, "heads": H, "dh": a.dh,
+                         "bytes": 4.0 * a.b * a.sq * H * (a.dh * (e + 1) + 4)}
+    q = torch.randn(a.b, a.sq, a.heads * a.dh, device=dev).to(ty)
+    o = torch.empty_like(q)
+    n = torch.full((a.b,), Lm, dtype=torch.int32, device=dev)
+    fn = lambda: L.call("dlm_attention_kv_i8", _p(q), a.heads * a.dh, *c, _p(o), a.heads * a.dh, a.b, a.heads, H,
+                        a.sq, a.dh, Lm, _p(n), None, 1, a.dh ** -0.5, t, _s())
+    seen = Lm - (a.sq - 1) / 2
+    return fn, 4.0 * a.b * a.heads * a.sq * seen * a.dh, {
+        "b": a.b, "heads": a.heads, "kv_heads": H, "sq": a.sq, "sk": Lm, "dh": a.dh,
+        "bytes": 2.0 * a.b * (H * Lm * (a.dh + 4) + a.sq * a.heads * a.dh * e)}
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("op", choices=["gemm", "conv", "attn", "ternary", "gn", "vae", "lm"])
+    ap.add_argument("op", choices=["gemm", "conv", "attn", "ternary", "gn", "vae", "lm",
+                                   "norm_i8", "gemm_i8", "kv_i8", "attn_i8"])
     ap.add_argument("--m", type=int, default=8192)
     ap.add_argument("--n", type=int, default=640)
     ap.add_argument("--k", type=int, default=640)
@@ -79,6 +132,9 @@ def main(argv=None):
     ap.add_argument("--sq", type=int, default=4096)
     ap.add_argument("--sk", type=int, default=4096)
     ap.add_argument("--dh", type=int, default=64, help="attention head dim (64, or 128..512)")
+    ap.add_argument("--kv-heads", type=int, default=0, help="attn_i8: kv heads (default: --heads)")
+    ap.add_argument("--dtype", choices=["f32", "f16", "bf16"], default="f16",
+                    help="element type of the int8 language-model operators")
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--eager", action="store_true",
                     help="time back-to-back ABI calls instead of a captured graph of them")
@@ -122,6 +178,8 @@ def main(argv=None):
         flops = 2.0 * a.m * a.n * a.k  # int8 ops
         shape = {"m": a.m, "n": a.n, "k": a.k,
                  "bytes": a.n * a.k / 4 + a.m * a.k + 4 * a.m * a.n + 4 * (a.m + a.n)}
+    elif a.op.endswith("_i8"):
+        fn, flops, shape = _int8_op(a, dev)
     elif a.op == "vae":
         from .vae import SDXLVAEDecoder, random_weights
         dec = SDXLVAEDecoder(random_weights(seed=9))
@@ -172,7 +230,8 @@ def main(argv=None):
                                 a.sq, a.sk, 64, 0.125, _p(ws), nws, _s())
         flops = 4.0 * a.b * a.heads * a.sq * a.sk * a.dh
         shape = {"b": a.b, "heads": a.heads, "sq": a.sq, "sk": a.sk, "dh": a.dh}
-    ms = _time_graph(fn, a.iters) if a.op in ("gemm", "attn", "gn") and not a.eager else _time(fn, a.iters)
+    ms = _time_graph(fn, a.iters) if (a.op in ("gemm", "attn", "gn") or
+                                     a.op.endswith("_i8")) and not a.eager else _time(fn, a.iters)
     peak = None
     pk = Path(__file__).resolve().parent.parent / "MEASURED_PEAKS.json"
     if pk.exists():
