@@ -93,7 +93,6 @@ def _int8_op(a, dev):
     Lm = a.sq if a.op == "kv_i8" else a.sk
     cache = [codes(a.b, H, Lm, a.dh), torch.rand(a.b, H, Lm, device=dev) / 64]
     cache += [c.clone() for c in cache]
-    c = [_p(x) for x in cache]
     if a.op == "kv_i8":
         k, v = (torch.randn(a.b, a.sq, H * a.dh, device=dev).to(ty) for _ in range(2))
         pos = torch.zeros(a.b, dtype=torch.int32, device=dev)
@@ -101,15 +100,15 @@ def _int8_op(a, dev):
         def fn():
             W = H * a.dh
             shape = (a.b, a.sq, H, a.dh, Lm, _p(pos), None, t, _s())
-            L.call("dlm_kv_i8_append", _p(k), W, _p(v), W, *c, *shape)
-            L.call("dlm_kv_i8_read", *c, _p(k), W, _p(v), W, *shape)
+            L.call("dlm_kv_i8_append", _p(k), W, _p(v), W, *map(_p, cache), *shape)
+            L.call("dlm_kv_i8_read", *map(_p, cache), _p(k), W, _p(v), W, *shape)
         return fn, 0.0, {"b": a.b, "s": a.sq, "heads": H, "dh": a.dh,
                          "bytes": 4.0 * a.b * a.sq * H * (a.dh * (e + 1) + 4)}
     q = torch.randn(a.b, a.sq, a.heads * a.dh, device=dev).to(ty)
     o = torch.empty_like(q)
     n = torch.full((a.b,), Lm, dtype=torch.int32, device=dev)
-    fn = lambda: L.call("dlm_attention_kv_i8", _p(q), a.heads * a.dh, *c, _p(o), a.heads * a.dh, a.b, a.heads, H,
-                        a.sq, a.dh, Lm, _p(n), None, 1, a.dh ** -0.5, t, _s())
+    fn = lambda: L.call("dlm_attention_kv_i8", _p(q), a.heads * a.dh, *map(_p, cache), _p(o), a.heads * a.dh, a.b,
+                        a.heads, H, a.sq, a.dh, Lm, _p(n), None, 1, a.dh ** -0.5, t, _s())
     seen = Lm - (a.sq - 1) / 2
     return fn, 4.0 * a.b * a.heads * a.sq * seen * a.dh, {
         "b": a.b, "heads": a.heads, "kv_heads": H, "sq": a.sq, "sk": Lm, "dh": a.dh,
