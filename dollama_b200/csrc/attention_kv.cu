@@ -568,6 +568,8 @@ extern "C" int dlm_attention_kv_i8(const void* q, int ldq, const int8_t* kq, con
               "attention_kv_i8: q / out rows must start on 16-byte boundaries");
   DLM_REQUIRE(aligned16(kq) && aligned16(vq), DLM_ERR_INVALID,
               "attention_kv_i8: cache codes must be 16-byte aligned");
+  DLM_REQUIRE(aligned4(kscale) && aligned4(vscale) && aligned4(kv_len) && aligned4(q_len), DLM_ERR_INVALID,
+              "attention_kv_i8: a scale or length array is not 4-byte aligned");
   DLM_REQUIRE(scale > -INFINITY && scale < INFINITY, DLM_ERR_INVALID, "attention_kv_i8: scale is not finite");
   const int g = Hq / Hkv;
   DLM_REQUIRE(static_cast<long long>(Sq) * g < (1ll << 30) && Lmax <= (1 << 30), DLM_ERR_UNSUPPORTED,

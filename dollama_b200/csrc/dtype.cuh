@@ -165,6 +165,7 @@ __device__ __forceinline__ int quant_exact(double x, double a) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 inline size_t dtype_size(int dtype) { return dtype == DLM_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == DLM_F32 || dtype == DLM_F16 || dtype == DLM_BF16; }
 

@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(kKvThreads)
 
 // The host checks of both calls; `empty` when there is nothing to do.
 int check(const char* fn, const void* k, int ldk, const void* v, int ldv, const void* kq, const void* ks,
-          const void* vq, const void* vs, int B, int S, int H, int Dh, int Lmax, const int* pos, int dtype,
-          bool& empty) {
+          const void* vq, const void* vs, int B, int S, int H, int Dh, int Lmax, const int* pos,
+          const int* counts, int dtype, bool& empty) {
   empty = false;
   DLM_REQUIRE(B >= 0 && S >= 0 && H >= 0 && Lmax >= 0, DLM_ERR_INVALID, "%s: negative size", fn);
   DLM_REQUIRE(dtype_ok(dtype), DLM_ERR_INVALID, "%s: unknown dtype %d", fn, dtype);
@@ -190,6 +190,8 @@ int check(const char* fn, const void* k, int ldk, const void* v, int ldv, const 
   DLM_REQUIRE(aligned16(k) && aligned16(v) && ldk % vec == 0 && ldv % vec == 0, DLM_ERR_INVALID,
               "%s: k / v rows must start on 16-byte boundaries", fn);
   DLM_REQUIRE(aligned16(kq) && aligned16(vq), DLM_ERR_INVALID, "%s: cache codes must be 16-byte aligned", fn);
+  DLM_REQUIRE(aligned4(ks) && aligned4(vs) && aligned4(pos) && aligned4(counts), DLM_ERR_INVALID,
+              "%s: a scale or position array is not 4-byte aligned", fn);
   DLM_REQUIRE(static_cast<double>(B) * S * H < 2147483000.0, DLM_ERR_UNSUPPORTED, "%s: too many rows", fn);
   return DLM_OK;
 }
@@ -215,7 +217,8 @@ int dlm_kv_i8_append(const void* k, int ldk, const void* v, int ldv, int8_t* kq,
                      const int* counts, int dtype, void* stream) {
   using namespace dlm;
   bool empty;
-  const int rc = check("kv_i8_append", k, ldk, v, ldv, kq, kscale, vq, vscale, B, S, H, Dh, Lmax, pos, dtype, empty);
+  const int rc = check("kv_i8_append", k, ldk, v, ldv, kq, kscale, vq, vscale, B, S, H, Dh, Lmax, pos, counts, dtype,
+                       empty);
   if (rc != DLM_OK || empty) return rc;
   const KvShape p = shape(B, S, H, Lmax, pos, counts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -232,7 +235,8 @@ int dlm_kv_i8_read(const int8_t* kq, const float* kscale, const int8_t* vq, cons
                    const int* counts, int dtype, void* stream) {
   using namespace dlm;
   bool empty;
-  const int rc = check("kv_i8_read", k, ldk, v, ldv, kq, kscale, vq, vscale, B, S, H, Dh, Lmax, pos, dtype, empty);
+  const int rc = check("kv_i8_read", k, ldk, v, ldv, kq, kscale, vq, vscale, B, S, H, Dh, Lmax, pos, counts, dtype,
+                       empty);
   if (rc != DLM_OK || empty) return rc;
   const KvShape p = shape(B, S, H, Lmax, pos, counts);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -59,7 +59,8 @@ CASES = [
         (dict(vq=None), INVALID), (dict(vs=None), INVALID), (dict(pos=None), INVALID), (dict(ldk=127), INVALID),
         (dict(ldv=64), INVALID), (dict(ldk=130), INVALID), (dict(k=A + 8), INVALID), (dict(vq=A + 8), INVALID),
         (dict(Dh=96, ldk=256, ldv=256), UNSUPPORTED), (dict(B=-1), INVALID), (dict(S=-2), INVALID),
-        (dict(Lm=-1), INVALID), (dict(t=5), INVALID))],
+        (dict(Lm=-1), INVALID), (dict(t=5), INVALID), (dict(ks=A + 2), INVALID), (dict(pos=A + 1), INVALID),
+        (dict(n=A + 2), INVALID), (dict(vs=A + 1), INVALID))],
     (attn, dict(q=None), INVALID), (attn, dict(o=None), INVALID), (attn, dict(kq=None), INVALID),
     (attn, dict(vs=None), INVALID), (attn, dict(n=None), INVALID), (attn, dict(Hkv=3), INVALID),
     (attn, dict(Hkv=0), INVALID), (attn, dict(ldq=255), INVALID), (attn, dict(ldo=252, Hq=4), INVALID),
@@ -67,6 +68,7 @@ CASES = [
     (attn, dict(scale=float("inf")), INVALID), (attn, dict(q=A + 4), INVALID), (attn, dict(t=1, ldq=260), INVALID),
     (attn, dict(B=-1), INVALID), (attn, dict(t=9), INVALID), (attn, dict(Lm=(1 << 30) + 1), UNSUPPORTED),
     (attn, dict(Sq=1 << 30), UNSUPPORTED),
+    (attn, dict(n=A + 2), INVALID), (attn, dict(m=A + 1), INVALID), (attn, dict(ks=A + 2), INVALID),
 ]
 
 

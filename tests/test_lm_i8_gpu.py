@@ -416,6 +416,28 @@ def test_attention_masked_keys_may_hold_anything(t, Sq):
 
 
 @pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("Sq", [3, 12, 40, 200])
+def test_attention_rows_are_independent(t, Sq):
+    """Infinite, NaN, huge and tiny queries leave the other rows' results as they are."""
+    g, ty = gen(21), O.TYPES[t]
+    q = torch.randn(1, Sq, 2, 64, generator=g, device="cuda").to(ty)
+    cache = make_cache(1, 1, 300, 64, g)
+    kv = torch.tensor([280], dtype=torch.int32, device="cuda")
+    clean = run_attn(q, cache, kv, None, True, t)
+    bad = q.clone()
+    bad[0, 0, 0, 3] = float("inf")
+    bad[0, 1, 1, 5] = float("nan")
+    bad[0, 2, 0] *= 1e4 if t == F16 else 1e30
+    bad[0, 2, 1] *= 1e-4 if t == F16 else 1e-30
+    out = run_attn(bad, cache, kv, None, True, t)
+    same_rows = [(i, h) for i in range(Sq) for h in range(2) if (i, h) not in ((0, 0), (1, 1), (2, 0), (2, 1))]
+    for i, h in same_rows:
+        assert torch.equal(out[0, i, h], clean[0, i, h]), (i, h)
+    assert torch.isnan(out[0, 0, 0]).all() and torch.isnan(out[0, 1, 1]).all()
+    check_attn(bad[:, 2:3, 1:], cache, torch.tensor([280 - Sq + 3], device="cuda"), None, True, t, out[:, 2:3, 1:])
+
+
+@pytest.mark.parametrize("t", ALL)
 @pytest.mark.parametrize("Sq", [1, 20, 140])
 def test_attention_scales_of_all_sizes(t, Sq):
     """Loud and silent rows: q, key and value scales over many orders of magnitude, sharp softmaxes."""
