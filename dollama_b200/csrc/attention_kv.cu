@@ -285,16 +285,18 @@ __global__ void __launch_bounds__(kThreads)
     else
       weigh(std::false_type{});
     if (__any_sync(0xffffffffu, big >= kMaxWeight || sum >= kMaxSum)) {
-      // the references move (the first unit, a score well above those so far, a large vscale)
+      // the references move (the first unit, a score well above those so far, a large vscale), each by
+      // its own row's need only: no row's result depends on its neighbours
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          float top = -INFINITY, top_w = -INFINITY;
+          float top = -INFINITY, top_w = -INFINITY, most = lu[n][z] >= kMaxSum ? INFINITY : 0.0f;
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+              most = fmaxf(most, fabsf(w[u][n][2 * h + z]));
               float& x = s[u][n][2 * h + z];
               x *= ksc[u][h] * qmul[n][z];
               if (k0 + 16 * u + gr + 8 * h >= lim[n][z]) x = -INFINITY;
@@ -305,8 +307,9 @@ __global__ void __launch_bounds__(kThreads)
           for (int x = 4; x <= 16; x <<= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             top_w = fmaxf(top_w, __shfl_xor_sync(0xffffffffu, top_w, x));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
           }
-          const float to = new_ref<T>(ref[n][z], top, top_w);
+          const float to = most >= kMaxWeight ? new_ref<T>(ref[n][z], top, top_w) : ref[n][z];
           const float alpha = fast_exp2(ref[n][z] - to);
           ref[n][z] = to;
           lu[n][z] = l[n][z] * alpha;
