@@ -510,8 +510,9 @@ int launch(AttnKvParams p, cudaStream_t s) {
   // tile and for clusters of 1 to 8 CTAs per tile (a cluster of 16, which needs
   // the kernel's leave, cost 7 us more to launch than it saved).
   constexpr double kFixed = 100.0;
+  const int sms = num_sms();
   auto cost = [&](long long ctas, int resident, int warps) {
-    const long long slots = static_cast<long long>(resident) * num_sms();
+    const long long slots = static_cast<long long>(resident) * sms;
     const long long units = (p.Lmax + static_cast<long long>(kUnit) * warps - 1) / (kUnit * warps);
     return static_cast<double>((ctas + slots - 1) / slots) * (static_cast<double>(units * kUnit) + kFixed);
   };
@@ -530,7 +531,7 @@ int launch(AttnKvParams p, cudaStream_t s) {
     return DLM_OK;
   }
   const unsigned grid = static_cast<unsigned>(tiles * p.C);
-  if (static_cast<long long>(grid) <= static_cast<long long>(per_few) * num_sms())
+  if (static_cast<long long>(grid) <= static_cast<long long>(per_few) * sms)
     DLM_CHECK_CUDA(launch_clusters(few, grid, kThreads, Few::kSmem, p.C, s, p));
   else
     DLM_CHECK_CUDA(launch_clusters(many, grid, kThreads, Many::kSmem, p.C, s, p));

@@ -615,10 +615,11 @@ int attn_kv_tc(const AttnKvParams& given, cudaStream_t s) {
   // CTAs per cluster: waves (one CTA per SM) times the longest row's keys, plus each CTA's fixed work
   // (about as long as kFixed keys), is least
   constexpr double kFixed = 512.0;
+  const int sms = num_sms();
   double best = 1e30;
   for (int c = 1; c <= 8; ++c) {
     const long long units = (p.Lmax + static_cast<long long>(KT) * c - 1) / (KT * c);
-    const double t = static_cast<double>((tiles * c + num_sms() - 1) / num_sms()) *
+    const double t = static_cast<double>((tiles * c + sms - 1) / sms) *
                      (static_cast<double>(units * KT) + kFixed);
     if (t < 0.97 * best) {
       best = t;

@@ -631,11 +631,10 @@ int launch(const int8_t* xq, long long ldx, const int8_t* w, GemmI8Params p, cud
 // Clusters of C CTAs that run at once (they have to fit inside the groups of SMs that share a cluster,
 // so this is less than the SMs divided by C).
 template <int NT, typename T>
-int resident_clusters(int C) {
+int resident_clusters(int C, int dev, int sms) {
   static int cache[64][4] = {{0}};
-  int dev = 0;
   const int i = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return num_sms() / C;
+  if (dev >= 64) return sms / C;
   if (cache[dev][i] == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(C);
@@ -651,7 +650,7 @@ int resident_clusters(int C) {
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_k_kernel<NT, T>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
-      n = num_sms() / C > 0 ? num_sms() / C : 1;
+      n = sms / C > 0 ? sms / C : 1;
     }
     cache[dev][i] = n;
   }
@@ -671,21 +670,21 @@ double tiles_of(int M, int N, int bm, int bn) {
 }
 
 // 128 x 128 tiles, one per SM: 512 x 512 x 512 5.1 us, 1024 x 8192 x 4096 35.8 us
-double estimate_single(int M, int N, int nkb) {
-  return 3.6 + std::ceil(tiles_of(M, N, 128, 128) / num_sms()) * (0.9 + 0.225 * nkb);
+double estimate_single(int M, int N, int nkb, int sms) {
+  return 3.6 + std::ceil(tiles_of(M, N, 128, 128) / sms) * (0.9 + 0.225 * nkb);
 }
 // 256 x 256 tiles, one per pair: 512 x 512 x 512 7.3 us, 1024 x 8192 x 4096 27.2 us
-double estimate_pair(int M, int N, int nkb) {
-  return 5.5 + std::ceil(tiles_of(M, N, 256, 256) / (num_sms() / 2)) * (2.8 + 0.29 * nkb);
+double estimate_pair(int M, int N, int nkb, int sms) {
+  return 5.5 + std::ceil(tiles_of(M, N, 256, 256) / (sms / 2)) * (2.8 + 0.29 * nkb);
 }
 // K split over clusters; up to NT tokens: 32 x 4096 x 4096 6.7 us (128 x 128 tiles: 10.8 us)
 template <int NT, typename T>
-Estimate estimate_k(int M, int N, int nkb) {
+Estimate estimate_k(int M, int N, int nkb, int dev, int sms) {
   constexpr double kFixed = NT == 16 ? 3.4 : NT == 32 ? 4.4 : NT == 64 ? 5.9 : 8.0;
   constexpr double kBlock = NT == 16 ? 0.127 : NT == 32 ? 0.14 : NT == 64 ? 0.17 : 0.225;
   Estimate best{1e30, 1};
   for (int C = 1; C <= 8 && (C == 1 || nkb >= 2 * C); C *= 2) {
-    const double waves = std::ceil(tiles_of(M, N, NT, 128) / resident_clusters<NT, T>(C));
+    const double waves = std::ceil(tiles_of(M, N, NT, 128) / resident_clusters<NT, T>(C, dev, sms));
     const double us = 2.0 + (C > 1 ? 0.3 : 0.0) + waves * (kFixed - 2.0 + ((nkb + C - 1) / C) * kBlock);
     if (us < best.us) best = Estimate{us, C};
   }
@@ -714,8 +713,11 @@ int launch_best(const int8_t* xq, long long ldx, const int8_t* w, const GemmI8Pa
   const int rc = allow_smem(gemm_i8_k_kernel<NT, T>, KCfg<NT>::kSmem, done);
   if (rc != DLM_OK) return rc;
   const int nkb = (p.K + kKB - 1) / kKB;
-  const double single = estimate_single(p.M, p.N, nkb), pair = estimate_pair(p.M, p.N, nkb);
-  const Estimate split = estimate_k<NT, T>(p.M, p.N, nkb);
+  const int sms = num_sms();
+  int dev = 0;
+  DLM_CHECK_CUDA(cudaGetDevice(&dev));
+  const double single = estimate_single(p.M, p.N, nkb, sms), pair = estimate_pair(p.M, p.N, nkb, sms);
+  const Estimate split = estimate_k<NT, T>(p.M, p.N, nkb, dev, sms);
   if (split.us <= single && split.us <= pair) return launch_k<NT, T>(xq, ldx, w, p, split.C, s);
   if (pair < single) return launch<true, T>(xq, ldx, w, p, s);
   return launch<false, T>(xq, ldx, w, p, s);
