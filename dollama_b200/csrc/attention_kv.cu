@@ -27,6 +27,11 @@
 // w_ij = p_ij vscale_j are taken against a reference of their row's own that keeps them in fp16's
 // range (so a key that a row does not see has no part in it) and rounded to fp16 (a relative error of
 // 2^-11 each), for fp32 split into two terms.  Sums are fp32.
+//
+// Bound by the cache's bytes once they are many: 64 sequences of up to 16384 tokens, 32 heads on 8, Dh
+// 128, fp16: 247-254 us, all of the measured copy rate; 8 of them 41 us (77 %: the start, the joins and
+// uneven lengths take 10).  A form with the queries as the instruction's 16 rows and loads straight into
+// fragments took 191 us there: half-empty tiles, and no loads in flight under the arithmetic.
 #include "attention_kv.cuh"
 
 namespace dlm {
