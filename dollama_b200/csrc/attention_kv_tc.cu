@@ -34,6 +34,12 @@ constexpr int kConvThreads = 128;
 
 constexpr int KT = 64;  // keys per tile
 
+// A cluster's CTAs wait for one another and for their tensor memory, all 512 columns.  Beside another
+// stream's clusters that hold some (dlm_gemm_i8's split-K kernel would fit next to the 119 KB of Dh 64)
+// each could hold the columns that the other's peer waits for, without end: so a CTA of a cluster takes
+// an SM's whole shared memory, and has the columns as soon as it runs.
+constexpr int kWholeSm = 227 * 1024;
+
 template <int DH, bool kSplit>
 struct TcCfg {
   static constexpr int NT = kSplit ? 2 : 1;  // fp16 terms of q and of the weights
@@ -460,6 +466,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tmem_st_16x256b_x4(to + h * kHalf + c, r);
             }
           }
+          tmem_st_wait();  // a second try reads O again
         }
       }
       if (!ok) break;
@@ -604,7 +611,7 @@ int attn_kv_tc(const AttnKvParams& given, cudaStream_t s) {
   DLM_CHECK_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !done[dev]) {
     DLM_CHECK_CUDA(cudaFuncSetAttribute(attn_kv_tc_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        C::kSmem));
+                                        kWholeSm));
     if (dev < 64) done[dev] = true;
   }
   const long long row_tiles = (static_cast<long long>(p.Sq) * p.g + kRows - 1) / kRows;
@@ -626,8 +633,9 @@ int attn_kv_tc(const AttnKvParams& given, cudaStream_t s) {
       p.C = c;
     }
   }
-  DLM_CHECK_CUDA(launch_clusters(attn_kv_tc_kernel<T, DH>, static_cast<unsigned>(tiles * p.C), kTcThreads, C::kSmem,
-                                 p.C, s, p));
+  const int smem = p.C > 1 ? kWholeSm : C::kSmem;
+  DLM_CHECK_CUDA(launch_clusters(attn_kv_tc_kernel<T, DH>, static_cast<unsigned>(tiles * p.C), kTcThreads, smem, p.C,
+                                 s, p));
   return DLM_OK;
 }
 

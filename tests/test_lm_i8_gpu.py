@@ -438,6 +438,25 @@ def test_attention_rows_are_independent(t, Sq):
 
 
 @pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("Sq,at", [(40, 291), (200, 200), (200, 270)])
+@pytest.mark.parametrize("Dh", [64, 128])
+def test_attention_tile_weighed_three_times(t, Sq, at, Dh):
+    """An infinite value scale late in the cache never fits: the rows that do not see its key keep their
+    results, whatever passes the tile takes for the others."""
+    g, ty = gen(23), O.TYPES[t]
+    q = torch.randn(1, Sq, 2, Dh, generator=g, device="cuda").to(ty)
+    cache = make_cache(1, 1, 300, Dh, g)
+    kv = torch.tensor([300], dtype=torch.int32, device="cuda")
+    clean = run_attn(q, cache, kv, None, True, t)
+    cache[3][0, 0, at] = float("inf")
+    out = run_attn(q, cache, kv, None, True, t)
+    n = at - (300 - Sq)  # query i sees keys 0 .. 300 - Sq + i
+    assert 0 < n < Sq
+    assert torch.equal(out[:, :n], clean[:, :n])
+    assert not torch.isfinite(out[:, n:]).any()
+
+
+@pytest.mark.parametrize("t", ALL)
 @pytest.mark.parametrize("Sq", [1, 20, 140])
 def test_attention_scales_of_all_sizes(t, Sq):
     """Loud and silent rows: q, key and value scales over many orders of magnitude, sharp softmaxes."""
@@ -589,6 +608,29 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for (o, (w, y), (_, _, _, a)) in zip(outs, want, work):
         assert torch.equal(o, w) and torch.equal(a[5], y)
+
+
+@pytest.mark.parametrize("M", [20, 33, 64])
+def test_split_product_beside_clusters_of_attention(M):
+    """Both kinds of clusters hold tensor memory: on two streams neither may keep the other's waiting."""
+    g = gen(60 + M)
+    q = torch.randn(4, 30, 4, 64, generator=g, device="cuda").half()
+    cache = make_cache(4, 2, 900, 64, g)
+    kv = torch.full((4,), 880, dtype=torch.int32, device="cuda")
+    a = make_gemm(M, 2048, 2048, F16, False, seed=M)
+    run_gemm(*a, F16, M, 2048, 2048)
+    want, y = run_attn(q, cache, kv, None, True, F16), a[5].clone()
+    a[5].fill_(-77)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    s = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(50):
+        with torch.cuda.stream(s[0]):
+            run_attn(q, cache, kv, None, True, F16, out=out)
+        with torch.cuda.stream(s[1]):
+            run_gemm(*a, F16, M, 2048, 2048)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(a[5], y)
 
 
 _FIRST = """
