@@ -20,7 +20,7 @@
 // each row scaled by a power of two for bf16 and fp32 (a row's result does not depend on its
 // neighbours).  For fp32 inputs q and the weights are two fp16 terms each, and every product is issued
 // for both.  Bound by the softmax and its hand-overs: 2 x 500 queries of 16 heads on 4 over 4096 keys,
-// bf16, 42 us, of which 31 us remain when the softmax does nothing but pass its tiles on; the
+// bf16, 44 us, of which 29 us remain when the softmax does nothing but pass its tiles on; the
 // exponentials alone take 10.
 #include "attention_kv.cuh"
 

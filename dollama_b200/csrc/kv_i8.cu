@@ -6,7 +6,7 @@
 // [B][H][Lmax][Dh], scales [B][H][Lmax], so a head's keys are contiguous for the attention that
 // reads them.  Neighbouring lanes take the K row and the V row of one token and head.  Memory-bound:
 // 16 sequences x 2048 tokens x 8 heads x 128, fp16, ragged: write 28.3 us (82 % of the measured copy
-// rate), read 27.9 us (84 %).  The write takes 32 bytes of a row a lane: with 16, the bookkeeping of a
+// rate), read 27.9 us (84 %) at best; both together 55 to 66 us from run to run.  The write takes 32 bytes of a row a lane: with 16, the bookkeeping of a
 // row (its place in the cache, the divisions by a and 127) took 38.8 us; the read takes 8 values a lane:
 // with 16, its 16-byte stores leave gaps between lanes (30.7 us).
 #include <cstdint>
