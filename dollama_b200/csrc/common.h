@@ -54,6 +54,18 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
 // Records the last host-side error message (thread-local), returned by dlm_last_error().
 void set_error(const char* fmt, ...);
 
+// Raises `kernel`'s dynamic shared-memory limit to `bytes`, once per device (`done`: the caller's own,
+// one for each kernel).
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && done[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
+
 }  // namespace dlm
 
 #define DLM_CHECK_CUDA(expr)                                                   \

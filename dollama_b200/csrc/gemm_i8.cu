@@ -569,17 +569,6 @@ constexpr CUtensorMapDataType tmap_type() {
                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
-// Raises a kernel's shared-memory limit, once per device.
-template <typename K>
-int allow_smem(K kernel, int bytes, bool (&done)[64]) {
-  int dev = 0;
-  DLM_CHECK_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && done[dev]) return DLM_OK;
-  DLM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  if (dev < 64) done[dev] = true;
-  return DLM_OK;
-}
-
 template <typename K, typename... Args>
 cudaError_t launch_cluster(K kernel, int grid, int threads, int smem, int cluster, cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};
@@ -603,8 +592,7 @@ template <bool kPair, typename T>
 int launch(const int8_t* xq, long long ldx, const int8_t* w, GemmI8Params p, cudaStream_t s) {
   using C = Cfg<kPair>;
   static bool done[64] = {false};
-  const int rc = allow_smem(gemm_i8_kernel<kPair, T>, C::kSmem, done);
-  if (rc != DLM_OK) return rc;
+  DLM_CHECK_CUDA(allow_smem(gemm_i8_kernel<kPair, T>, C::kSmem, done));
   CUtensorMap tx, tw, ty{};
   if (!tmap_i8(&tx, xq, p.M, p.K, ldx, kBM) || !tmap_i8(&tw, w, p.N, p.K, p.K, 128)) return DLM_ERR_CUDA;
   if (p.y_tma) {
@@ -710,8 +698,7 @@ int launch_k(const int8_t* xq, long long ldx, const int8_t* w, GemmI8Params p, i
 template <int NT, typename T>
 int launch_best(const int8_t* xq, long long ldx, const int8_t* w, const GemmI8Params& p, cudaStream_t s) {
   static bool done[64] = {false};
-  const int rc = allow_smem(gemm_i8_k_kernel<NT, T>, KCfg<NT>::kSmem, done);
-  if (rc != DLM_OK) return rc;
+  DLM_CHECK_CUDA(allow_smem(gemm_i8_k_kernel<NT, T>, KCfg<NT>::kSmem, done));
   const int nkb = (p.K + kKB - 1) / kKB;
   const int sms = num_sms();
   int dev = 0;

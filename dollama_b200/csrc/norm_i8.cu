@@ -247,9 +247,10 @@ int launch_norm(const NormParams& p, cudaStream_t s) {
     const int threads = n >= 2048 ? 512 : n >= 512 ? 256 : (n + 31) / 32 * 32;
     const size_t smem = static_cast<size_t>((n + threads - 1) / threads) * threads * VEC * sizeof(T);
     auto kernel = add_rms_norm_i8_kernel<T, VEC, 0>;
-    if (smem > 48 * 1024)
-      DLM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          static_cast<int>((kNormMaxK + 512) * sizeof(T))));
+    // always: the static arrays share the 48 KB that a kernel has without leave, so a row of just that
+    // size needs it too
+    static bool done[64] = {false};
+    DLM_CHECK_CUDA(allow_smem(kernel, static_cast<int>((kNormMaxK + 512) * sizeof(T)), done));
     DLM_CHECK_CUDA(launch_pdl(kernel, dim3(p.M), dim3(threads), smem, s, p));
   }
   return DLM_OK;

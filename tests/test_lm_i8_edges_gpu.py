@@ -1,0 +1,49 @@
+"""The int8 language-model operators where their launch rules and main loops change form: rows just
+below a kernel's shared-memory limit, rings used many times over, references that move late, keys and
+rows that must not touch one another.  Tolerances and 64-bit forms are those of test_lm_i8_gpu."""
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+from dollama_b200 import _lib as L
+from tests import lm_i8_oracle as O
+from tests import test_lm_i8_gpu as G
+from tests.test_lm_i8_gpu import ALL, F32, clean_status, gen  # noqa: F401 (clean_status: autouse)
+
+pytestmark = pytest.mark.gpu
+ROOT = str(Path(__file__).resolve().parent.parent)
+
+
+def fresh_process(code):
+    """Runs `code` in a process of its own, in which it makes the first calls of the library."""
+    r = subprocess.run([sys.executable, "-c", code, ROOT], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert r.returncode == 0 and "done" in r.stdout, r.stdout + r.stderr
+
+
+# ------------------------------------------------------------------ norm
+
+_LONG_ROWS = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from tests import test_lm_i8_gpu as G
+ty = torch.%s
+for K in %s:
+    g = G.gen(K)
+    x, r = ((torch.randn(2, K, generator=g, device="cuda")).to(ty) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(K, generator=g, device="cuda")).to(ty)
+    G.check_norm(x, r, w, G.run_norm(x, r, w))
+print("done")
+"""
+
+
+@pytest.mark.parametrize("ty,Ks", [("float32", (10244, 12288)), ("float32", (11777, 12287)),
+                                   ("float16", (20488, 24576)), ("float16", (24065, 24575)),
+                                   ("bfloat16", (20488, 24576)), ("bfloat16", (24065, 24575))])
+def test_norm_rows_of_48_kilobytes_first(ty, Ks):
+    """Rows that take 48 KB of dynamic shared memory (beside the kernel's static arrays) as a process's
+    first: no longer row has raised the kernel's limit before."""
+    fresh_process(_LONG_ROWS % (ty, Ks))
