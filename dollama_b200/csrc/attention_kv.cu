@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(kThreads)
       weigh(std::false_type{});
     if (__any_sync(0xffffffffu, big >= kMaxWeight || sum >= kMaxSum)) {
       // the references move (the first unit, a score well above those so far, a large vscale), each by
-      // its own row's need only: no row's result depends on its neighbours
+      // its own row's need only; a row that stays keeps the weights it has (formed again as below they
+      // would differ by a rounding): no row's result depends on its neighbours, to the bit
 #pragma unroll
       for (int n = 0; n < NR; ++n)
 #pragma unroll
@@ -314,18 +315,21 @@ __global__ void __launch_bounds__(kThreads)
             top_w = fmaxf(top_w, __shfl_xor_sync(0xffffffffu, top_w, x));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
           }
-          const float to = most >= kMaxWeight ? new_ref<T>(ref[n][z], top, top_w) : ref[n][z];
+          const bool moves = most >= kMaxWeight;
+          const float to = moves ? new_ref<T>(ref[n][z], top, top_w) : ref[n][z];
           const float alpha = fast_exp2(ref[n][z] - to);
           ref[n][z] = to;
-          lu[n][z] = l[n][z] * alpha;
+          float lm = l[n][z] * alpha;
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float e = fast_exp2(s[u][n][2 * h + z] - to);
-              lu[n][z] += e;
-              w[u][n][2 * h + z] = k0 + 16 * u + gr + 8 * h >= lim[n][z] ? 0.0f : e * vsc[u][h];
+              const float wm = k0 + 16 * u + gr + 8 * h >= lim[n][z] ? 0.0f : e * vsc[u][h];
+              lm += e;
+              if (moves) w[u][n][2 * h + z] = wm;
             }
+          if (moves) lu[n][z] = lm;
 #pragma unroll
           for (int j = 0; j < KS; ++j) {
             o[n][j][z] *= alpha;

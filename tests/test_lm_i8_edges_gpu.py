@@ -47,3 +47,24 @@ def test_norm_rows_of_48_kilobytes_first(ty, Ks):
     """Rows that take 48 KB of dynamic shared memory (beside the kernel's static arrays) as a process's
     first: no longer row has raised the kernel's limit before."""
     fresh_process(_LONG_ROWS % (ty, Ks))
+
+
+# ------------------------------------------------------------------ attention: rows and keys apart
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("Sq,Lm,B", [(2, 4096, 1), (4, 4096, 1), (8, 4096, 1), (4, 100, 900), (8, 100, 900)])
+def test_few_rows_keep_their_bits_when_a_neighbour_moves(t, Dh, Sq, Lm, B):
+    """A loud key that the last query alone sees, in a unit of keys that is not its warp's first (one
+    sequence: four units of a warp, clusters; 900: a warp each): the last query's reference moves, the
+    other rows' results stay to the bit."""
+    g, ty = gen(Sq + Dh), O.TYPES[t]
+    q = (1.5 * torch.randn(B, Sq, 2, Dh, generator=g, device="cuda")).to(ty)
+    cache = G.make_cache(B, 1, Lm, Dh, g)
+    n = Lm - 6  # the last unit holds keys that all see, too
+    kv = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    clean = G.run_attn(q, cache, kv, None, True, t)
+    cache[3][:, :, n - 1] *= 1e6
+    out = G.run_attn(q, cache, kv, None, True, t)
+    assert torch.equal(out[:, :Sq - 1], clean[:, :Sq - 1])
+    assert not torch.equal(out[:, Sq - 1], clean[:, Sq - 1])
