@@ -59,6 +59,9 @@ struct TcCfg {
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
+// Weights from here on do not say how far their reference is too low (they may have overflowed).
+constexpr float kFarWeight = 1e30f;
+
 // 16 codes -> 16 fp16 values (two 16-byte pieces)
 __device__ __forceinline__ void expand16(uint4 c, uint4& a, uint4& b) {
   const uint32_t x = c.x ^ 0x80808080u, y = c.y ^ 0x80808080u, z = c.z ^ 0x80808080u, w = c.w ^ 0x80808080u;
@@ -376,8 +379,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       };
       // References move each by its own row's need only (a row that fits keeps its weights), and the
-      // tile is weighed again, twice at most (infinite scores or scales never fit).  A finite overshoot
-      // says how far; the first tile, scores or scales far beyond, and a second try ask for the maxima.
+      // tile is weighed again, twice at most (infinite scores or scales never fit).  On the first try an
+      // overshoot below kFarWeight says how far and rows beyond it wait; on the second, rows that still do
+      // not fit ask for the maxima, as all do on the first tile.  So the way a row's reference takes, and
+      // with it the rounding of its weights, depends on no other row.
       bool search = n == 0;
       for (int tries = 0;; ++tries) {
         if (!search) {
@@ -396,9 +401,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           for (int y = 0; y < 4; ++y) {
             big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 1));
             big[y] = fmaxf(big[y], __shfl_xor_sync(0xffffffffu, big[y], 2));
-            search = search || (big[y] >= kMaxWeight && !(tries == 0 && big[y] < 1e30f));
           }
-          search = __any_sync(0xffffffffu, search);
+          search = tries > 0;
         } else {
 #pragma unroll
           for (int y = 0; y < 4; ++y) big[y] = INFINITY;
@@ -439,7 +443,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         } else {
 #pragma unroll
           for (int y = 0; y < 4; ++y)
-            alpha[y] = big[y] >= kMaxWeight ? ref[y] + __log2f(big[y]) - kTarget<T> : ref[y];
+            alpha[y] = big[y] >= kMaxWeight && big[y] < kFarWeight ? ref[y] + __log2f(big[y]) - kTarget<T> : ref[y];
         }
 #pragma unroll
         for (int y = 0; y < 4; ++y) {

@@ -68,3 +68,23 @@ def test_few_rows_keep_their_bits_when_a_neighbour_moves(t, Dh, Sq, Lm, B):
     out = G.run_attn(q, cache, kv, None, True, t)
     assert torch.equal(out[:, :Sq - 1], clean[:, :Sq - 1])
     assert not torch.equal(out[:, Sq - 1], clean[:, Sq - 1])
+
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("loud", [1e5, 1e36])
+def test_many_rows_keep_their_bits_when_a_neighbour_searches(t, Dh, loud):
+    """Keys late in the cache (ten tiles, one CTA for all of them): one whose weight overshoots every
+    row's reference by a known factor, one that only the last query sees and that sends its row back for
+    the tile's maxima.  The other rows move as they do alone, to the bit."""
+    g, ty = gen(Dh), O.TYPES[t]
+    B, Hkv, Sq, Lm = 37, 4, 20, 640  # 148 row tiles
+    q = (1.5 * torch.randn(B, Sq, Hkv, Dh, generator=g, device="cuda")).to(ty)
+    cache = G.make_cache(B, Hkv, Lm, Dh, g)
+    cache[3][:, :, Lm - 30] *= 1e5
+    kv = torch.full((B,), Lm, dtype=torch.int32, device="cuda")
+    clean = G.run_attn(q, cache, kv, None, True, t)
+    cache[3][:, :, Lm - 1] *= loud
+    out = G.run_attn(q, cache, kv, None, True, t)
+    assert torch.equal(out[:, :Sq - 1], clean[:, :Sq - 1])
+    assert not torch.equal(out[:, Sq - 1], clean[:, Sq - 1])
