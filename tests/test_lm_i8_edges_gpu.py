@@ -88,3 +88,78 @@ def test_many_rows_keep_their_bits_when_a_neighbour_searches(t, Dh, loud):
     out = G.run_attn(q, cache, kv, None, True, t)
     assert torch.equal(out[:, :Sq - 1], clean[:, :Sq - 1])
     assert not torch.equal(out[:, Sq - 1], clean[:, Sq - 1])
+
+
+# ------------------------------------------------------------------ attention: long runs of the main loops
+
+def shaped_cache(B, Hkv, Lm, Dh, shape, q, g):
+    """smooth: random codes; rising: keys turn towards the queries along the cache, so that the scores'
+    maximum moves again and again; leaps: a few keys far above (2^100 and more) all before them; values:
+    value scales grow along the cache by 2^36; falling: the first keys are the loudest."""
+    cache = G.make_cache(B, Hkv, Lm, Dh, g)
+    j = torch.arange(Lm, device="cuda") / Lm
+    if shape in ("rising", "falling"):
+        to = q.float().mean((1, 2))  # [B, Dh], shared by all queries (see base below)
+        to = 90 * to / to.abs().amax(-1, keepdim=True)
+        a = j if shape == "rising" else 1 - j
+        k = a[:, None] * to[:, None, None] + (1 - a[:, None]) * cache[0].float() * 0.4
+        cache[0].copy_(k.round().clamp(-127, 127))
+        cache[1].mul_(5)
+    elif shape == "leaps":
+        cache[1][:, :, Lm * 2 // 5::97] *= 40
+    elif shape == "values":
+        cache[3].mul_(torch.exp2(36 * j - 30))
+    return cache
+
+
+def check_some(q, cache, kv, causal, t, out, seqs, queries):
+    """Query i alone is the last of a shorter sequence."""
+    Sq = q.shape[1]
+    s = torch.tensor(seqs, device="cuda")
+    for i in queries:
+        n = kv[s] - (Sq - 1 - i if causal else 0)
+        G.check_attn(q[s, i:i + 1].contiguous(), [c[s] for c in cache], n, None, causal, t,
+                     out[s, i:i + 1])
+
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("shape", ["smooth", "rising", "falling", "leaps", "values"])
+@pytest.mark.parametrize("B,Hkv,g,Sq,Lm", [(37, 4, 2, 20, 700), (19, 4, 2, 70, 460), (1, 4, 1, 20, 8000)])
+def test_many_rows_over_many_tiles(t, Dh, shape, B, Hkv, g, Sq, Lm):
+    """The many-row kernel with 8 to 16 tiles of 64 keys a CTA (row tiles for every SM, two waves of them,
+    and a cluster of eight), so that stages, score buffers and phases are used again and O is rescaled
+    between tiles: rising and values move a row's reference 1.7 to 3.6 times after a stream's first tile,
+    leaps half of them, some beyond what an overshoot can say (counted on the inputs in 64 bits)."""
+    gn, ty = gen(B + Sq + Dh), O.TYPES[t]
+    base = torch.randn(B, 1, 1, Dh, generator=gn, device="cuda")
+    noise = torch.randn(B, Sq, Hkv * g, Dh, generator=gn, device="cuda")
+    q = (base + 0.5 * noise if shape in ("rising", "falling") else 1.5 * noise).to(ty)
+    cache = shaped_cache(B, Hkv, Lm, Dh, shape, q, gn)
+    kv = torch.randint(Lm - 100, Lm + 1, (B,), generator=gn, device="cuda", dtype=torch.int32)
+    for c in (cache[1], cache[3]):
+        for b in range(B):
+            c[b, :, int(kv[b]):] = float("nan")
+    for causal in (True, False):
+        out = G.run_attn(q, cache, kv, None, causal, t)
+        check_some(q, cache, kv, causal, t, out, sorted({0, B // 2, B - 1}), (0, Sq // 2, Sq - 1))
+        assert torch.equal(out, G.run_attn(q, cache, kv, None, causal, t))
+
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("shape", ["smooth", "rising", "falling", "leaps", "values"])
+@pytest.mark.parametrize("B,Hkv,g,Sq,Lm", [(1, 1, 8, 1, 16000), (1, 2, 4, 4, 16000), (150, 2, 4, 1, 900),
+                                           (600, 2, 2, 2, 500)])
+def test_few_rows_over_many_units(t, Dh, shape, B, Hkv, g, Sq, Lm):
+    """The few-row kernel with 7 to 16 units of 32 keys a warp: clusters with the deep ring, one or two CTAs
+    a tile with the shallow one, a warp a tile."""
+    gn, ty = gen(B + Sq + Dh), O.TYPES[t]
+    base = torch.randn(B, 1, 1, Dh, generator=gn, device="cuda")
+    noise = torch.randn(B, Sq, Hkv * g, Dh, generator=gn, device="cuda")
+    q = (base + 0.5 * noise if shape in ("rising", "falling") else 1.5 * noise).to(ty)
+    cache = shaped_cache(B, Hkv, Lm, Dh, shape, q, gn)
+    kv = torch.randint(Lm - 100, Lm + 1, (B,), generator=gn, device="cuda", dtype=torch.int32)
+    out = G.run_attn(q, cache, kv, None, True, t)
+    check_some(q, cache, kv, True, t, out, sorted({0, B // 2, B - 1}), (0, Sq - 1) if Sq > 1 else (0,))
+    assert torch.equal(out, G.run_attn(q, cache, kv, None, True, t))
