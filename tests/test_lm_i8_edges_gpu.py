@@ -163,3 +163,36 @@ def test_few_rows_over_many_units(t, Dh, shape, B, Hkv, g, Sq, Lm):
     out = G.run_attn(q, cache, kv, None, True, t)
     check_some(q, cache, kv, True, t, out, sorted({0, B // 2, B - 1}), (0, Sq - 1) if Sq > 1 else (0,))
     assert torch.equal(out, G.run_attn(q, cache, kv, None, True, t))
+
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("Sq", [4, 8, 150])
+@pytest.mark.parametrize("Lm,B", [(300, 1), (4096, 1), (300, 500)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_keys_of_later_queries_may_hold_anything(t, Dh, Sq, Lm, B, what):
+    """NaN and infinite key and value scales of keys that the last two queries alone see: 8 and 16 rows of
+    the few-row kernel (clusters of one and of four units a warp, a warp a tile) and 300 rows."""
+    if B > 1 and Sq > 8:
+        B = 60  # row tiles beyond a wave
+    g, ty = gen(Sq + Lm), O.TYPES[t]
+    q = torch.randn(B, Sq, 2, Dh, generator=g, device="cuda").to(ty)
+    cache = G.make_cache(B, 1, Lm, Dh, g)
+    n = Lm - 3
+    kv = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    clean = G.run_attn(q, cache, kv, None, True, t)
+    before = Sq - 2
+    assert before > 0
+    for ks, vs in ((what, None), (None, what), (what, what)):
+        bad = [c.clone() for c in cache]
+        for at in (n - 2, n - 1):
+            if ks is not None:
+                bad[1][:, :, at] = ks
+            if vs is not None:
+                bad[3][:, :, at] = vs
+        out = G.run_attn(q, bad, kv, None, True, t)
+        assert torch.equal(out[:, :before], clean[:, :before])
+        # a key's NaN is its row's; an infinite key scale is a score of +-inf (a weight of NaN or 0), an
+        # infinite value scale a result that is not finite
+        if what != what or vs is not None:
+            assert not torch.isfinite(out[:, Sq - 1]).any()
