@@ -196,3 +196,69 @@ def test_keys_of_later_queries_may_hold_anything(t, Dh, Sq, Lm, B, what):
         # infinite value scale a result that is not finite
         if what != what or vs is not None:
             assert not torch.isfinite(out[:, Sq - 1]).any()
+
+
+# ------------------------------------------------------------------ first calls captured
+
+_CAPTURED = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from tests import test_lm_i8_gpu as G
+dev = dict(device="cuda")
+g = G.gen(1)
+K = %d
+x = torch.randn(40, K, generator=g, **dev).half()
+w = torch.ones(K, **dev).half()
+wq = torch.randint(-127, 128, (256, 256), generator=g, device="cuda", dtype=torch.int8)
+ws = torch.rand(256, generator=g, **dev)
+xq = torch.randint(-127, 128, (40, 256), generator=g, device="cuda", dtype=torch.int8)
+xs = torch.rand(40, generator=g, **dev) / 64  # sums of 256 products of 73 x 73, about 9e4, inside fp16
+pos = torch.zeros(2, dtype=torch.int32, **dev)
+kv = torch.full((2,), 20, dtype=torch.int32, **dev)
+qq = torch.randn(2, 20, 4, 64, generator=g, **dev).half()
+q1 = qq[:, :1].contiguous()
+out = dict(h=torch.empty_like(x), q=torch.empty(40, K, dtype=torch.int8, **dev), s=torch.empty(40, **dev),
+           y=torch.empty(40, 256, **dev).half(), kq=torch.empty(2, 2, 64, 64, dtype=torch.int8, **dev),
+           ks=torch.empty(2, 2, 64, **dev), vq=torch.empty(2, 2, 64, 64, dtype=torch.int8, **dev),
+           vs=torch.empty(2, 2, 64, **dev), k=torch.empty(2, 20, 2, 64, **dev).half(),
+           v=torch.empty(2, 20, 2, 64, **dev).half(), many=torch.empty_like(qq), one=torch.empty_like(q1))
+cache = [out[n] for n in ("kq", "ks", "vq", "vs")]
+def fill():
+    for o in out.values():
+        o.fill_(99)
+def all_of_them():
+    G.L.call("dlm_add_rms_norm_i8", x.data_ptr(), K, None, 0, w.data_ptr(), out["h"].data_ptr(), K,
+             out["q"].data_ptr(), out["s"].data_ptr(), 40, K, 1e-5, 1, G._s())
+    G.run_gemm(xq, xs, wq, ws, None, out["y"], 1, 40, 256, 256)
+    G.L.call("dlm_kv_i8_append", out["y"].data_ptr(), 256, out["y"].data_ptr() + 256, 256,
+             *[c.data_ptr() for c in cache], 2, 20, 2, 64, 64, pos.data_ptr(), None, 1, G._s())
+    G.read(out["k"], out["v"], cache, pos, None, 1, 64)
+    G.run_attn(qq, cache, kv, None, True, 1, out=out["many"])
+    G.run_attn(q1, cache, kv, None, True, 1, out=out["one"])
+fill()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    all_of_them()
+torch.cuda.synchronize()
+assert all((o == 99).all() for o in out.values())  # captured, not run
+graph.replay()
+torch.cuda.synchronize()
+got = {n: o.clone() for n, o in out.items()}
+fill()
+all_of_them()
+torch.cuda.synchronize()
+for n, o in out.items():
+    assert torch.equal(got[n], o) and torch.isfinite(o).all(), n
+    assert (o != 99).any(), n
+G.check_norm(x, None, w, (got["h"], got["q"], got["s"]))
+G.check_attn(q1, cache, kv, None, True, 1, got["one"])
+print("done")
+"""
+
+
+@pytest.mark.parametrize("K", [256, 24575])
+def test_every_first_call_captured(K):
+    """Each operator's first call of a process in a capture (norm rows in registers and in shared memory,
+    many and few rows of attention): what the replay writes is what the eager calls write."""
+    fresh_process(_CAPTURED % K)
