@@ -348,7 +348,8 @@ int dlm_bitnet_weight_info(const dlm_bitnet_config* cfg, int index, char* name, 
  * x, residual, weight and h_out are of `dtype`; xq is [M, K] contiguous, xscale [M].  h is rounded
  * to `dtype` before it is normed.  Codes are exact: those of the formula without roundings
  * (fp32 inputs: with the products in double).  K <= 32768, eps > 0, any alignment of the elements;
- * rows that all start on 16-byte boundaries are faster. */
+ * rows that all start on 16-byte boundaries are faster.  With M or K == 0 nothing is written,
+ * xscale neither. */
 int dlm_add_rms_norm_i8(const void* x, int ldx, const void* residual, int ldr, const void* weight,
                         void* h_out, int ldh, int8_t* xq, float* xscale, int M, int K, float eps,
                         int dtype, void* stream);
@@ -358,7 +359,7 @@ int dlm_add_rms_norm_i8(const void* x, int ldx, const void* residual, int ldr, c
  * xq [M, K] (row stride ldx), w [N, K] contiguous, xscale [M], wscale [N], bias [N] of `dtype` or
  * NULL, y [M, N] of `dtype` (row stride ldy; the elements between rows stay).  The integer sum is
  * exact, the epilogue fp32.  K and ldx multiples of 16, K < 131072, xq and w 16-byte aligned;
- * any M and N. */
+ * any M and N.  K == 0 is an empty problem as any size of 0 is: y is not written, a bias neither. */
 int dlm_gemm_i8(const int8_t* xq, int ldx, const float* xscale, const int8_t* w, const float* wscale,
                 const void* bias, void* y, int ldy, int M, int N, int K, int dtype, void* stream);
 

@@ -49,6 +49,35 @@ def test_norm_rows_of_48_kilobytes_first(ty, Ks):
     fresh_process(_LONG_ROWS % (ty, Ks))
 
 
+# ------------------------------------------------------------------ empty problems
+
+@pytest.mark.parametrize("t", ALL)
+def test_a_size_of_zero_writes_nothing(t):
+    """Any size of 0 is an empty problem: no output changes, a product's bias with K = 0 included."""
+    ty = O.TYPES[t]
+    p, s = G._p, G._s()
+    x, w = torch.ones(4, 64, device="cuda", dtype=ty), torch.ones(64, device="cuda", dtype=ty)
+    h, xq, xs = (torch.full((4, 64), 9, device="cuda", dtype=d) for d in (ty, torch.int8, torch.float32))
+    for M, K in ((0, 64), (4, 0), (0, 0)):
+        L.call("dlm_add_rms_norm_i8", p(x), 64, None, 0, p(w), p(h), 64, p(xq), p(xs), M, K, 1e-5, t, s)
+    wq, y = torch.ones(32, 64, device="cuda", dtype=torch.int8), torch.full((4, 32), 9, device="cuda", dtype=ty)
+    for M, N, K in ((4, 32, 0), (0, 32, 64), (4, 0, 64)):
+        L.call("dlm_gemm_i8", p(xq), 64, p(xs), p(wq), p(xs), p(w), p(y), 32, M, N, K, t, s)
+    cache = G.empty_cache(2, 2, 16, 64)
+    k = torch.full((2, 3, 2, 64), 9, device="cuda", dtype=ty)
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for B, S, H, Lm in ((0, 3, 2, 16), (2, 0, 2, 16), (2, 3, 0, 16), (2, 3, 2, 0)):
+        shape = (B, S, H, 64, Lm, p(pos), None, t, s)
+        L.call("dlm_kv_i8_append", p(k), 128, p(k), 128, *map(p, cache), *shape)
+        L.call("dlm_kv_i8_read", *map(p, cache), p(k), 128, p(k), 128, *shape)
+    o = torch.full((2, 3, 4, 64), 9, device="cuda", dtype=ty)
+    for B, Hq, Hkv, Sq in ((0, 4, 2, 3), (2, 0, 2, 3), (2, 4, 2, 0)):
+        L.call("dlm_attention_kv_i8", p(k), 256, *map(p, cache), p(o), 256, B, Hq, Hkv, Sq, 64, 16, p(pos), None, 1,
+               0.125, t, s)
+    assert all((z == 9).all() for z in (h, xq, xs, y, k, o))
+    assert all((c == v).all() for c, v in zip(cache, (55, 9, 55, 9)))
+
+
 # ------------------------------------------------------------------ attention: rows and keys apart
 
 @pytest.mark.parametrize("t", ALL)
