@@ -588,7 +588,8 @@ extern "C" int dlm_attention_kv_i8(const void* q, int ldq, const int8_t* kq, con
   DLM_REQUIRE(static_cast<long long>(Sq) * g < (1ll << 30) && Lmax <= (1 << 30), DLM_ERR_UNSUPPORTED,
               "attention_kv_i8: too many rows or cache positions");
   const AttnKvParams p{q, kq, kscale, vq, vscale, out, kv_len, q_len, ldq, ldo, B, Hq, Hkv, Sq, Lmax, g,
-                       1, 1, causal, 1, scale * 1.4426950408889634f, device_status_ptr()};
+                       1, 1, causal, 1, scale * 1.4426950408889634f, device_status_ptr(),
+                       device_position_ptr()};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DLM_DISPATCH_DTYPE(dtype, T, {
     if (Dh == 64) return launch_rows<T, 64>(p, s);

@@ -27,6 +27,7 @@ struct AttnKvParams {
   int C;          // CTAs of a cluster, which share one tile's keys
   float scale_log2;
   int* status;
+  int* bad_position;  // device status word of lengths outside the cache
 };
 
 // Rows above which the tensor-memory kernel runs.
@@ -36,7 +37,7 @@ template <typename T, int DH>
 int attn_kv_tc(const AttnKvParams& p, cudaStream_t s);
 
 // One (sequence, kv head, row tile): its rows r0 .. last (row r: query r / g, head r % g) and the keys
-// they see.  A length outside the cache is clamped and raises the device status word.
+// they see.  A length outside the cache is clamped and raises the device status word of positions.
 struct AttnKvTile {
   int b, hkv, r0, last, n_kv, n_q, n_keys, n_all;
 
@@ -47,7 +48,7 @@ struct AttnKvTile {
     b = t / p.Hkv;
     n_kv = p.kv_len[b];
     if (n_kv < 0 || n_kv > p.Lmax) {
-      if (report && p.status) atomicCAS(p.status, 0, kDevBadPosition);
+      if (report && p.bad_position) *p.bad_position = kDevBadPosition;
       n_kv = n_kv < 0 ? 0 : p.Lmax;
     }
     n_q = p.q_len ? p.q_len[b] : p.Sq;

@@ -12,9 +12,10 @@ namespace {
 
 thread_local char g_last_error[1024] = "";
 
-// Status word written by kernels that give up a bounded wait.  One per device (each device
+// Status words: [0] written by kernels that give up a bounded wait, [1] by kernels that were given a
+// position outside a cache (apart, so that neither hides the other).  One pair per device (each device
 // that loads the library holds its own copy of this variable).
-__device__ int g_dlm_device_status = 0;
+__device__ int g_dlm_device_status[2] = {0, 0};
 
 constexpr int kMaxDevices = 64;
 
@@ -67,6 +68,11 @@ int* device_status_ptr() {
     cache[dev] = static_cast<int*>(p);
   }
   return cache[dev];
+}
+
+int* device_position_ptr() {
+  int* p = device_status_ptr();
+  return p ? p + 1 : nullptr;
 }
 
 bool encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, const void* base,
@@ -133,15 +139,16 @@ int dlm_get_device_status(int* out_code, int clear, void* stream) {
   int* p = dlm::device_status_ptr();
   DLM_REQUIRE(p != nullptr, DLM_ERR_CUDA, "dlm_get_device_status: no device status symbol");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int v = 0;
-  DLM_CHECK_CUDA(cudaMemcpyAsync(&v, p, sizeof(int), cudaMemcpyDeviceToHost, s));
+  int v[2] = {0, 0};
+  DLM_CHECK_CUDA(cudaMemcpyAsync(v, p, sizeof(v), cudaMemcpyDeviceToHost, s));
   DLM_CHECK_CUDA(cudaStreamSynchronize(s));
-  if (clear && v != 0) {
+  const int word = v[0] != 0 ? 0 : 1;
+  if (clear && v[word] != 0) {  // the other word waits for the next call
     const int zero = 0;
-    DLM_CHECK_CUDA(cudaMemcpyAsync(p, &zero, sizeof(int), cudaMemcpyHostToDevice, s));
+    DLM_CHECK_CUDA(cudaMemcpyAsync(p + word, &zero, sizeof(int), cudaMemcpyHostToDevice, s));
     DLM_CHECK_CUDA(cudaStreamSynchronize(s));
   }
-  *out_code = v;
+  *out_code = v[word];
   return DLM_OK;
 }
 

@@ -17,6 +17,8 @@ int num_sms();
 // Device address of this library's status word on the current device (kernels that give
 // up a bounded wait record a nonzero code there).  Cached per device.
 int* device_status_ptr();
+// The word beside it, for kernels that were given a position outside a cache (kDevBadPosition).
+int* device_position_ptr();
 
 // cuTensorMapEncodeTiled through cudaGetDriverEntryPoint (no link-time libcuda dependency).
 // Returns false if the driver rejects the map.

@@ -35,7 +35,7 @@ struct KvShape {
   int B, S, H, Lmax;
   const int* pos;     // [B] position of each sequence's first new token
   const int* counts;  // [B] new tokens of each sequence, or null: S
-  int* status;        // device status word
+  int* bad_position;  // device status word of positions
   unsigned units;     // B * S * H
   FastDiv by_h, by_s;
 };
@@ -62,7 +62,7 @@ struct Part {
 };
 
 // Unit u is (token, head).  Whether its cache row exists: the token is below its sequence's count and
-// its position inside the cache (a position outside raises the device status word).
+// its position inside the cache (a position outside raises the device status word of positions).
 __device__ __forceinline__ bool locate(const KvShape& p, unsigned u, unsigned& tok, unsigned& hd, size_t& row) {
   if (u >= p.units) return false;
   tok = p.by_h.div(u);
@@ -72,7 +72,7 @@ __device__ __forceinline__ bool locate(const KvShape& p, unsigned u, unsigned& t
   if (s >= (p.counts ? p.counts[b] : p.S)) return false;
   const long long at = static_cast<long long>(p.pos[b]) + s;
   if (at < 0 || at >= p.Lmax) {
-    if (p.status) atomicCAS(p.status, 0, kDevBadPosition);
+    if (p.bad_position) *p.bad_position = kDevBadPosition;
     return false;
   }
   row = (static_cast<size_t>(b) * p.H + hd) * p.Lmax + static_cast<size_t>(at);
@@ -197,7 +197,7 @@ int check(const char* fn, const void* k, int ldk, const void* v, int ldv, const 
 }
 
 KvShape shape(int B, int S, int H, int Lmax, const int* pos, const int* counts) {
-  return KvShape{B, S, H, Lmax, pos, counts, device_status_ptr(), static_cast<unsigned>(B) * S * H,
+  return KvShape{B, S, H, Lmax, pos, counts, device_position_ptr(), static_cast<unsigned>(B) * S * H,
                  FastDiv(H), FastDiv(S)};
 }
 

@@ -16,7 +16,8 @@ namespace dlm {
 
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s
 
-// Error codes written to dlm_device_status by a kernel that gave up waiting.
+// Error codes written to the device status words by a kernel that gave up waiting, or (the last, in a
+// word of its own) that was given a bad position.
 enum DeviceStatus : int {
   kDevOk = 0,
   kDevTimeoutProducer = 1,

@@ -52,10 +52,11 @@ const char* dlm_last_error(void);
 /* Library version string. */
 const char* dlm_version(void);
 
-/* Reads (and clears when `clear` != 0) the device status word of the current device:
- * 0 = no kernel gave up a wait; 1..5 = the code of the first kernel role that timed out; 6 = an
- * int8 cache call was given a position or a length outside its cache (those rows were skipped).
- * Synchronizes `stream`. */
+/* Reads (and clears when `clear` != 0) the device status of the current device: 1..5 = the code of
+ * the first kernel role that gave up a wait; 6 = no kernel did, but an int8 cache call was given a
+ * position or a length outside its cache (append and read skipped that row, the attention took the
+ * length as 0 or Lmax); 0 = neither.  Where both happened, a call that clears the first leaves the
+ * 6 to the next.  Synchronizes `stream`. */
 int dlm_get_device_status(int* out_code, int clear, void* stream);
 
 /* Asynchronous copy between any two (device or host) buffers on `stream`. */

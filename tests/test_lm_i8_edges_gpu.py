@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from dollama_b200 import _lib as L
+from dollama_b200.build import nvcc
 from tests import lm_i8_oracle as O
 from tests import test_lm_i8_gpu as G
 from tests.test_lm_i8_gpu import ALL, F32, clean_status, gen  # noqa: F401 (clean_status: autouse)
@@ -291,3 +292,64 @@ def test_every_first_call_captured(K):
     """Each operator's first call of a process in a capture (norm rows in registers and in shared memory,
     many and few rows of attention): what the replay writes is what the eager calls write."""
     fresh_process(_CAPTURED % K)
+
+
+# ------------------------------------------------------------------ device status
+
+_STATUS = r"""
+#include "dollama_b200/csrc/common.cu"
+#include "dollama_b200/csrc/attention_kv.cuh"
+using namespace dlm;
+// a barrier that nothing arrives on: the wait gives up after its two seconds
+__global__ void give_up(int* status) {
+  __shared__ uint64_t bar;
+  __shared__ int abort_flag;
+  abort_flag = 0;
+  mbar_init(&bar, 1);
+  fence_mbar_init();
+  mbar_wait(&bar, 0, &abort_flag, status, kDevTimeoutMma);
+}
+// the attention's own check of a length outside its cache
+__global__ void bad_length(const AttnKvParams p) { AttnKvTile(p, 0, 8, true); }
+int read(int clear) {
+  int c = -1;
+  return dlm_get_device_status(&c, clear, nullptr) == DLM_OK ? c : -2;
+}
+int main() {
+  const int five = 5;
+  int* n = nullptr;
+  if (cudaMalloc(&n, 4) != cudaSuccess || cudaMemcpy(n, &five, 4, cudaMemcpyHostToDevice) != cudaSuccess) return 1;
+  AttnKvParams p{};
+  p.kv_len = n;
+  p.Lmax = 4;
+  p.Sq = p.Hkv = p.Hq = p.g = p.B = p.row_tiles = p.tiles = 1;
+  p.status = device_status_ptr();
+  p.bad_position = device_position_ptr();
+  printf("%d ", read(1));
+  bad_length<<<1, 1>>>(p);
+  printf("%d ", read(0));
+  printf("%d ", read(1));
+  printf("%d ", read(1));
+  bad_length<<<1, 1>>>(p);
+  give_up<<<1, 1>>>(p.status);
+  bad_length<<<1, 1>>>(p);
+  printf("%d ", read(0));
+  printf("%d ", read(1));
+  printf("%d ", read(1));
+  printf("%d\n", read(1));
+  return cudaDeviceSynchronize() == cudaSuccess ? 0 : 1;
+}
+"""
+
+
+def test_a_bad_length_does_not_hide_a_timeout(tmp_path):
+    """A kernel that gave up a wait is reported whatever bad positions came before it; they are reported
+    after it."""
+    src, exe = tmp_path / "status.cu", tmp_path / "status"
+    src.write_text(_STATUS.replace("\n#include \"", "\n#include \"" + ROOT + "/"))
+    r = subprocess.run([nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17",
+                        "--expt-relaxed-constexpr", "-I", ROOT + "/include", "-o", str(exe), str(src)],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.split() == "0 6 6 0 2 2 6 0".split(), r.stdout + r.stderr
