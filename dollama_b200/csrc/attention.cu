@@ -646,13 +646,16 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
           float mmax = m_run;
           for (int cc = first; cc <= last; ++cc)
             if (cc != me) mmax = fmaxf(mmax, __ldcg(p.part_ml + static_cast<size_t>(slot_of(cc)) * kQ + r_in).x);
-          // own O is unnormalised (sum of 2^((s - m) c) v): its weight l 2^((m - M) c) over l
-          const float so = fast_exp2((m_run - mmax) * c);
-          float L = l_run * so;
+          // The arithmetic is the counted path's to the bit (this piece is the block's first; its O
+          // normalised and rounded to fp16 as it would have been in the workspace): which path runs
+          // goes by the CTAs' timing, and the result must not.
+          const float own = __fmul_rn(l_run, fast_exp2((m_run - mmax) * c));
+          const float inv_l = 1.0f / l_run;
+          float L = own;
           for (int cc = first; cc <= last; ++cc) {
             if (cc == me) continue;
             const float2 ml = __ldcg(p.part_ml + static_cast<size_t>(slot_of(cc)) * kQ + r_in);
-            L += ml.y * fast_exp2((ml.x - mmax) * c);
+            L = __fadd_rn(L, __fmul_rn(ml.y, fast_exp2((ml.x - mmax) * c)));
           }
           const float inv = 1.0f / L;
 #pragma unroll 1
@@ -662,14 +665,19 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
             tmem_ld_wait();
             float a16[16];
 #pragma unroll
-            for (int d = 0; d < 16; ++d) a16[d] = __uint_as_float(r[d]) * so;
+            for (int d = 0; d < 16; d += 2) {
+              const uint32_t h = pack_half2(__uint_as_float(r[d]) * inv_l, __uint_as_float(r[d + 1]) * inv_l);
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+              a16[d] = fmaf(own, f.x, 0.0f);
+              a16[d + 1] = fmaf(own, f.y, 0.0f);
+            }
             for (int cc = first; cc <= last; ++cc) {
               if (cc == me) continue;
               const size_t sl = static_cast<size_t>(slot_of(cc)) * kQ + r_in;
               const float2 ml = __ldcg(p.part_ml + sl);
               const uint4* po = reinterpret_cast<const uint4*>(p.part_o + sl * kD) + 2 * qd;
               const uint4 o0 = __ldcg(po), o1 = __ldcg(po + 1);
-              const float w = ml.y * fast_exp2((ml.x - mmax) * c);
+              const float w = __fmul_rn(ml.y, fast_exp2((ml.x - mmax) * c));
               const __half2* h0 = reinterpret_cast<const __half2*>(&o0);
               const __half2* h1 = reinterpret_cast<const __half2*>(&o1);
 #pragma unroll
@@ -769,8 +777,8 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
             uint4 ov[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) ov[j] = __ldcg(po + j);
-            const float w = ml.y * fast_exp2((ml.x - mmax) * c);
-            L += w;
+            const float w = __fmul_rn(ml.y, fast_exp2((ml.x - mmax) * c));
+            L = __fadd_rn(L, w);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const __half2* hh = reinterpret_cast<const __half2*>(&ov[j]);
