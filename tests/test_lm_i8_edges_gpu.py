@@ -50,6 +50,43 @@ def test_norm_rows_of_48_kilobytes_first(ty, Ks):
     fresh_process(_LONG_ROWS % (ty, Ks))
 
 
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("K", [8200, 12288, 24575, 32768])
+@pytest.mark.parametrize("over", ["x", "residual"])
+def test_norm_long_rows_in_place(t, K, over):
+    """Rows in shared memory whose sum replaces an input."""
+    g, ty = gen(K), O.TYPES[t]
+    x, r = (torch.randn(3, K, generator=g, device="cuda").to(ty) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(K, generator=g, device="cuda")).to(ty)
+    x0, r0 = x.clone(), r.clone()
+    got = G.run_norm(x, r, w, h=x if over == "x" else r)
+    G.check_norm(x0, r0, w, got)
+    assert torch.equal(r, r0) if over == "x" else torch.equal(x, x0)
+
+
+def test_norm_and_product_beyond_32_bit_offsets():
+    """More than 2^31 elements in rows and results: the last rows."""
+    M, K = 70000, 32768
+    g = gen(77)
+    x = torch.empty(M, K, device="cuda", dtype=torch.half)
+    x.normal_(generator=g)
+    w = (1 + 0.2 * torch.randn(K, generator=g, device="cuda")).half()
+    h, q, s = G.run_norm(x, None, w)
+    for rows in (slice(0, 2), slice(65535, 65538), slice(M - 2, M)):
+        G.check_norm(x[rows], None, w, (h[rows], q[rows], s[rows]))
+    del x, h
+    N = 32768
+    a = q[:, :256].contiguous()
+    wq = torch.randint(-127, 128, (N, 256), generator=g, device="cuda", dtype=torch.int8)
+    ws = torch.rand(N, generator=g, device="cuda") / 64
+    for t, ldy in ((L.F16, N), (L.BF16, N + 1)):  # tensor stores, element stores
+        y = torch.full((M, ldy), -77.0, device="cuda", dtype=O.TYPES[t])
+        G.run_gemm(a, s, wq, ws, None, y, t, M, N, 256)
+        for rows in (slice(0, 2), slice(65534, 65538), slice(M - 2, M)):
+            G.check_gemm(a[rows], s[rows], wq, ws, None, y[rows], t, len(a[rows]), N, 256)
+        del y
+
+
 # ------------------------------------------------------------------ empty problems
 
 @pytest.mark.parametrize("t", ALL)
@@ -353,3 +390,18 @@ def test_a_bad_length_does_not_hide_a_timeout(tmp_path):
     assert r.returncode == 0, r.stderr
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and r.stdout.split() == "0 6 6 0 2 2 6 0".split(), r.stdout + r.stderr
+
+
+# ------------------------------------------------------------------ attention: any finite scale
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-6, 4.0])
+@pytest.mark.parametrize("Sq", [1, 8, 40])
+def test_attention_scale(t, scale, Sq):
+    """No weight but equal ones, the lowest scores first, and rows that one key takes."""
+    g, ty = gen(Sq), O.TYPES[t]
+    q = torch.randn(2, Sq, 4, 64, generator=g, device="cuda").to(ty)
+    cache = G.make_cache(2, 2, 200, 64, g)
+    kv = torch.tensor([200, 77], dtype=torch.int32, device="cuda")
+    out = G.run_attn(q, cache, kv, None, True, t, scale=scale)
+    G.check_attn(q, cache, kv, None, True, t, out, scale=scale)
