@@ -30,7 +30,14 @@ struct AttnKvParams {
   int* bad_position;  // device status word of lengths outside the cache
 };
 
-// Rows above which the tensor-memory kernel runs.
+// Rows (queries times heads of a group) above which the tensor-memory kernel runs: as many as the
+// few-row kernel holds in registers.  Its tile of 64 keys costs about the same for 17 rows as for 128.
+// 4 sequences, 8 kv heads, 16384 keys, fp16, us (cache bytes alone 11 / 21 for Dh 64 / 128):
+//   rows                                       16         24         32         64        128
+//   few-row kernel, a tile for every 16   23 / 35    35 / 56    36 / 56   59 / 100  124 / 177
+//   tensor-memory kernel                              71 / 97    71 / 98    72 / 99   74 / 102
+// and with 16 sequences of 512 keys 11 / 16 against 14 / 18 for 24 rows, 20 / 29 against 14 / 19 for
+// 128: with long caches the border would lie nearer to 64 rows, with short ones at 32.
 constexpr int kAttnKvFewRows = 16;
 
 template <typename T, int DH>

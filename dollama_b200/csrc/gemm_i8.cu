@@ -10,9 +10,11 @@
 //                      pair (cta_group::2) per 256 x 256 tile, or a CTA per 128 x 128 tile.  Bound by
 //                      the tensor cores and the power limit for large K (8192 x 8192 x 4096, fp16 out:
 //                      177 us, 3100 TOP/s; with one CTA per 128 x 128 tile 329 us, bound by operand
-//                      reads from L2: 128 bytes a clock and SM asked for, about 64 served), by the
-//                      epilogue's conversions and the output's bytes for small K (4096 x 16000 x 512:
-//                      48 us for 137 MB);
+//                      reads from L2, by their count: 128 bytes a clock and SM asked for).  Small K is
+//                      far from both floors (4096 x 16000 x 512, fp16 out: 49 us, 22 by the bytes, 20
+//                      by the operations; fp32 out 74 for 42): latencies of the epilogue, little of
+//                      which four k-blocks hide (tensor pipe 34 %, issue slots 35 %, DRAM 19 %).  Odd
+//                      N stores by elements: 1003 x 2111 x 1360 bf16 11.0 us, N = 2112 10.0;
 //   gemm_i8_k_kernel   for few tokens: 128 channels (the MMA's M operand) x up to 128 tokens per
 //                      cluster, whose CTAs split K and add their integer partial sums over
 //                      distributed shared memory (integers: any order gives the same sum).  Bound by

@@ -20,8 +20,9 @@ namespace {
 
 constexpr int kKvThreads = 256;
 
-// n / d for n < 2^31 by a multiplication: q = (umulhi(n, mul) + n) >> shift with shift =
-// ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, "Division by Invariant Integers using
+// Multiplication", 1994): q = (umulhi(n, mul) + n) >> shift with shift = ceil(log2 d), mul =
+// floor(2^32 (2^shift - d) / d) + 1.
 struct FastDiv {
   unsigned d, mul, shift;
   explicit FastDiv(unsigned v) : d(v), mul(0), shift(0) {

@@ -388,8 +388,9 @@ int dlm_kv_i8_read(const int8_t* kq, const float* kscale, const int8_t* vq, cons
  * that sees no key gets zeros; queries from q_len[b] on are not written; keys that a query does not
  * see do not touch its result, whatever they hold.  A kv_len outside [0, Lmax] is clamped and
  * raises the device status word (code 6); a q_len above Sq counts as Sq, below 0 as 0.  kv_len,
- * q_len: device int32 [B].  Dh 64 or 128; Lmax <= 2^30; q and out rows on 16-byte boundaries.  Softmax statistics and sums are fp32; fp32 inputs keep 22 bits or
- * more of q and of the weights, 16-bit inputs 11 of the weights. */
+ * q_len: device int32 [B].  Dh 64 or 128; Lmax <= 2^30; q and out rows on 16-byte boundaries.
+ * Softmax statistics and sums are fp32; fp32 inputs keep 22 bits or more of q and of the weights,
+ * 16-bit inputs 11 of the weights.  The launch goes by Lmax, as the lengths are on the device. */
 int dlm_attention_kv_i8(const void* q, int ldq, const int8_t* kq, const float* kscale,
                         const int8_t* vq, const float* vscale, void* out, int ldo, int B, int Hq,
                         int Hkv, int Sq, int Dh, int Lmax, const int* kv_len, const int* q_len,
