@@ -612,8 +612,9 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
       const int qrow = q0 + t * kQT + row;
       __half* dst = p.out + static_cast<size_t>(b) * p.o_sb + static_cast<size_t>(h) * p.o_sh +
                     static_cast<size_t>(qrow) * p.o_ss;
-      // a group cut between CTAs (stream-K): this piece goes to the workspace, normalised by its
-      // own row sum, and the last CTA to finish merges the pieces
+      // a group cut between CTAs (stream-K): this piece goes to the workspace, in fp16 normalised by
+      // its own row sum (the group's first piece: unnormalised in fp32, as it is in TMEM), and the
+      // last CTA to finish merges the pieces
       // a cut query block (stream-K); with one key tile per block (not kSplit) none is ever cut
       const bool piece = kSK && kSplit && !sg.whole;
       const int r_in = t * kQT + row;
@@ -624,8 +625,8 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
         last = attn_cta_of(total, p.sk_ctas, static_cast<long long>(sg.group + 1) * n_tiles - 1);
       }
       auto slot_of = [&](int cc) { return 2 * cc + (cc == first ? 1 : 0); };
-      const size_t my_slot = static_cast<size_t>(slot_of(static_cast<int>(blockIdx.x))) * kQ + r_in;
-      if (piece && sg.j0 == 0) {
+      const bool head = piece && sg.j0 == 0;
+      if (head) {
         // The last piece of a cut query block, when every other piece is already in the workspace
         // (their CTAs have counted them): merge straight from this CTA's O in TMEM, without
         // writing and re-reading its own piece.  This CTA does not count itself, so no other can
@@ -646,16 +647,15 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
           float mmax = m_run;
           for (int cc = first; cc <= last; ++cc)
             if (cc != me) mmax = fmaxf(mmax, __ldcg(p.part_ml + static_cast<size_t>(slot_of(cc)) * kQ + r_in).x);
-          // The arithmetic is the counted path's to the bit (this piece is the block's first; its O
-          // normalised and rounded to fp16 as it would have been in the workspace): which path runs
-          // goes by the CTAs' timing, and the result must not.
-          const float own = __fmul_rn(l_run, fast_exp2((m_run - mmax) * c));
-          const float inv_l = 1.0f / l_run;
-          float L = own;
+          // own O is unnormalised (sum of 2^((s - m) c) v): its weight l 2^((m - M) c) over l.  The
+          // counted path below does the same arithmetic: which of the two runs goes by the CTAs'
+          // timing, and the bits of the result must not.
+          const float so = fast_exp2((m_run - mmax) * c);
+          float L = __fmul_rn(l_run, so);
           for (int cc = first; cc <= last; ++cc) {
             if (cc == me) continue;
             const float2 ml = __ldcg(p.part_ml + static_cast<size_t>(slot_of(cc)) * kQ + r_in);
-            L = __fadd_rn(L, __fmul_rn(ml.y, fast_exp2((ml.x - mmax) * c)));
+            L = fmaf(ml.y, fast_exp2((ml.x - mmax) * c), L);
           }
           const float inv = 1.0f / L;
 #pragma unroll 1
@@ -665,17 +665,12 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
             tmem_ld_wait();
             float a16[16];
 #pragma unroll
-            for (int d = 0; d < 16; d += 2) {
-              const uint32_t h = pack_half2(__uint_as_float(r[d]) * inv_l, __uint_as_float(r[d + 1]) * inv_l);
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-              a16[d] = fmaf(own, f.x, 0.0f);
-              a16[d + 1] = fmaf(own, f.y, 0.0f);
-            }
+            for (int d = 0; d < 16; ++d) a16[d] = __uint_as_float(r[d]) * so;
             for (int cc = first; cc <= last; ++cc) {
               if (cc == me) continue;
-              const size_t sl = static_cast<size_t>(slot_of(cc)) * kQ + r_in;
-              const float2 ml = __ldcg(p.part_ml + sl);
-              const uint4* po = reinterpret_cast<const uint4*>(p.part_o + sl * kD) + 2 * qd;
+              const float2 ml = __ldcg(p.part_ml + static_cast<size_t>(slot_of(cc)) * kQ + r_in);
+              const uint4* po =
+                  reinterpret_cast<const uint4*>(p.part_o + (static_cast<size_t>(cc) * kQ + r_in) * kD) + 2 * qd;
               const uint4 o0 = __ldcg(po), o1 = __ldcg(po + 1);
               const float w = __fmul_rn(ml.y, fast_exp2((ml.x - mmax) * c));
               const __half2* h0 = reinterpret_cast<const __half2*>(&o0);
@@ -712,8 +707,20 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
       {
         // O leaves TMEM 32 columns at a time (fp16, scaled by 1 / l), then the next segment's
         // first P.V may overwrite it
+        if (head) {
+          uint4* ph = reinterpret_cast<uint4*>(p.part_head + (static_cast<size_t>(blockIdx.x) * kQ + r_in) * kD);
+#pragma unroll 1
+          for (int qd = 0; qd < 4; ++qd) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(to + qd * 16, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              __stcg(ph + 4 * qd + j, make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]));
+          }
+        }
         const float inv = 1.0f / l_run;
-        uint4* po = reinterpret_cast<uint4*>(p.part_o + my_slot * kD);
+        if (!head) {
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           uint32_t r[32];
@@ -728,6 +735,7 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
             v[j].w = pack_half2(__uint_as_float(r[8 * j + 6]) * inv, __uint_as_float(r[8 * j + 7]) * inv);
           }
           if (piece) {
+            uint4* po = reinterpret_cast<uint4*>(p.part_o + (static_cast<size_t>(blockIdx.x) * kQ + r_in) * kD);
 #pragma unroll
             for (int j = 0; j < 4; ++j) __stcg(po + 4 * hf + j, v[j]);
           } else if (qrow < p.Sq) {
@@ -735,11 +743,13 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
             for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + 32 * hf + 8 * j) = v[j];
           }
         }
+        }
         tc_fence_before();
         mbar_arrive(&o_empty[t]);
       }
       if (!piece) continue;
-      __stcg(p.part_ml + my_slot, make_float2(m_run, l_run));
+      __stcg(p.part_ml + static_cast<size_t>(slot_of(static_cast<int>(blockIdx.x))) * kQ + r_in,
+             make_float2(m_run, l_run));
       __threadfence();
       ok = ep_meet();
       if (!ok) break;
@@ -751,9 +761,9 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
       if (!ok) break;
       if (*last_flag) {
         __threadfence();
-        // merge the pieces in CTA order: O = sum_s w_s O_s / sum_s w_s, w_s = l_s 2^((m_s - m) c),
-        // 32 columns at a time; the (max, sum) pairs of up to four pieces are requested before
-        // any is used
+        // merge the pieces in CTA order: O = sum_s w_s O_s / sum_s w_s, w_s = l_s 2^((m_s - m) c)
+        // (the first piece's O_s is l_s times that), 16 columns at a time; the (max, sum) pairs of up
+        // to four pieces are requested before any is used
         float mmax = -INFINITY;
         for (int c0 = first; c0 <= last; c0 += 4) {
           float2 m4[4];
@@ -764,42 +774,51 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
           for (int i = 0; i < 4; ++i)
             if (c0 + i <= last) mmax = fmaxf(mmax, m4[i].x);
         }
+        const float2 ml0 = __ldcg(p.part_ml + static_cast<size_t>(slot_of(first)) * kQ + r_in);
+        const float so = fast_exp2((ml0.x - mmax) * c);
 #pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-          float a32[32];
+        for (int qd = 0; qd < 4; ++qd) {
+          float a16[16];
+          float L = __fmul_rn(ml0.y, so);
+          const float4* ph =
+              reinterpret_cast<const float4*>(p.part_head + (static_cast<size_t>(first) * kQ + r_in) * kD) + 4 * qd;
 #pragma unroll
-          for (int d = 0; d < 32; ++d) a32[d] = 0.0f;
-          float L = 0.0f;
-          for (int cc = first; cc <= last; ++cc) {
-            const size_t sl = static_cast<size_t>(slot_of(cc)) * kQ + r_in;
-            const float2 ml = __ldcg(p.part_ml + sl);
-            const uint4* po = reinterpret_cast<const uint4*>(p.part_o + sl * kD) + 4 * hf;
-            uint4 ov[4];
+          for (int j = 0; j < 4; ++j) {
+            const float4 f = __ldcg(ph + j);
+            a16[4 * j] = f.x * so;
+            a16[4 * j + 1] = f.y * so;
+            a16[4 * j + 2] = f.z * so;
+            a16[4 * j + 3] = f.w * so;
+          }
+          for (int cc = first + 1; cc <= last; ++cc) {
+            const float2 ml = __ldcg(p.part_ml + static_cast<size_t>(slot_of(cc)) * kQ + r_in);
+            const uint4* po =
+                reinterpret_cast<const uint4*>(p.part_o + (static_cast<size_t>(cc) * kQ + r_in) * kD) + 2 * qd;
+            const uint4 ov[2] = {__ldcg(po), __ldcg(po + 1)};
+            const float e = fast_exp2((ml.x - mmax) * c);
+            const float w = __fmul_rn(ml.y, e);
+            L = fmaf(ml.y, e, L);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ov[j] = __ldcg(po + j);
-            const float w = __fmul_rn(ml.y, fast_exp2((ml.x - mmax) * c));
-            L = __fadd_rn(L, w);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
               const __half2* hh = reinterpret_cast<const __half2*>(&ov[j]);
 #pragma unroll
               for (int k2 = 0; k2 < 4; ++k2) {
                 const float2 f = __half22float2(hh[k2]);
-                a32[8 * j + 2 * k2] = fmaf(w, f.x, a32[8 * j + 2 * k2]);
-                a32[8 * j + 2 * k2 + 1] = fmaf(w, f.y, a32[8 * j + 2 * k2 + 1]);
+                a16[8 * j + 2 * k2] = fmaf(w, f.x, a16[8 * j + 2 * k2]);
+                a16[8 * j + 2 * k2 + 1] = fmaf(w, f.y, a16[8 * j + 2 * k2 + 1]);
               }
             }
           }
           if (qrow < p.Sq) {
             const float inv = 1.0f / L;
 #pragma unroll
-            for (int d = 0; d < 32; d += 8) {
+            for (int d = 0; d < 16; d += 8) {
               uint4 v;
-              v.x = pack_half2(a32[d] * inv, a32[d + 1] * inv);
-              v.y = pack_half2(a32[d + 2] * inv, a32[d + 3] * inv);
-              v.z = pack_half2(a32[d + 4] * inv, a32[d + 5] * inv);
-              v.w = pack_half2(a32[d + 6] * inv, a32[d + 7] * inv);
-              *reinterpret_cast<uint4*>(dst + 32 * hf + d) = v;
+              v.x = pack_half2(a16[d] * inv, a16[d + 1] * inv);
+              v.y = pack_half2(a16[d + 2] * inv, a16[d + 3] * inv);
+              v.z = pack_half2(a16[d + 4] * inv, a16[d + 5] * inv);
+              v.w = pack_half2(a16[d + 6] * inv, a16[d + 7] * inv);
+              *reinterpret_cast<uint4*>(dst + 16 * qd + d) = v;
             }
           }
         }
@@ -841,8 +860,8 @@ size_t attn_counter_bytes(int B, int H, int Sq) {
 }
 
 size_t attn_workspace_bytes(int B, int H, int Sq) {
-  const size_t slots = 2 * static_cast<size_t>(num_sms());
-  return attn_counter_bytes(B, H, Sq) + slots * kQ * sizeof(float2) + slots * kQ * kD * sizeof(__half);
+  const size_t rows = static_cast<size_t>(num_sms()) * kQ;
+  return attn_counter_bytes(B, H, Sq) + rows * (2 * sizeof(float2) + kD * (sizeof(__half) + sizeof(float)));
 }
 
 int attn_plan(AttnOp* op, int B, int H, int Sq, int Sk, int Dh, float scale, const AttnTensor& q,
@@ -887,6 +906,8 @@ int attn_plan(AttnOp* op, int B, int H, int Sq, int Sk, int Dh, float scale, con
     p.part_ml = reinterpret_cast<float2*>(base);
     base += 2 * static_cast<size_t>(sms) * kQ * sizeof(float2);
     p.part_o = reinterpret_cast<__half*>(base);
+    base += static_cast<size_t>(sms) * kQ * kD * sizeof(__half);
+    p.part_head = reinterpret_cast<float*>(base);
     op->grid = p.sk_ctas;
   }
   return DLM_OK;

@@ -21,14 +21,15 @@ struct AttnParams {
   long long o_sb, o_sh, o_ss;
   int* status;
   // stream-K (sk_ctas > 0, grid == sk_ctas): the groups' KV tile-steps are split evenly over the
-  // CTAs; every segment of a group cut between CTAs leaves its normalised O rows (fp16) and
-  // (row max, row sum) in slot 2 * cta + (cta holds the group's first tiles ? 1 : 0), and the CTA
-  // that finishes the group last (arrival counter part_cnt[group], zero between launches) merges
-  // the slots in CTA order.
+  // CTAs; every segment of a group cut between CTAs leaves its O rows (normalised in fp16; the
+  // group's first segment as accumulated, in fp32) in its CTA's place and (row max, row sum) in slot
+  // 2 * cta + (cta holds the group's first tiles ? 1 : 0), and the CTA that finishes the group last
+  // (arrival counter part_cnt[group], zero between launches) merges the pieces in CTA order.
   int sk_ctas;
-  __half* part_o;   // [2 * sk_ctas][256][64]
-  float2* part_ml;  // [2 * sk_ctas][256]
-  int* part_cnt;    // [groups]
+  __half* part_o;    // [SMs][256][64]
+  float* part_head;  // [SMs][256][64] first segments
+  float2* part_ml;   // [2 * SMs][256]
+  int* part_cnt;     // [groups]
 };
 
 struct AttnOp {

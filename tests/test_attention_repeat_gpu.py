@@ -1,7 +1,7 @@
 """The load-balanced flash attention gives the same bits whatever the timing of its CTAs (GPU).
 
 A query block cut between CTAs is merged by the one that finishes last, from the workspace or, for the
-block's first piece, partly from tensor memory: both ways have to be the same arithmetic."""
+block's first piece, partly from tensor memory: both ways are the same arithmetic."""
 import ctypes
 
 import pytest
