@@ -705,8 +705,8 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
         }
       }
       {
-        // O leaves TMEM 32 columns at a time (fp16, scaled by 1 / l), then the next segment's
-        // first P.V may overwrite it
+        // O leaves TMEM (a group's first piece as it is, else in fp16 scaled by 1 / l), then the next
+        // segment's first P.V may overwrite it
         if (head) {
           uint4* ph = reinterpret_cast<uint4*>(p.part_head + (static_cast<size_t>(blockIdx.x) * kQ + r_in) * kD);
 #pragma unroll 1
@@ -718,31 +718,30 @@ __global__ void __launch_bounds__(attn_threads(kSplit), 1)
             for (int j = 0; j < 4; ++j)
               __stcg(ph + 4 * qd + j, make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]));
           }
-        }
-        const float inv = 1.0f / l_run;
-        if (!head) {
+        } else {
+          const float inv = 1.0f / l_run;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(to + hf * 32, r);
-          tmem_ld_wait();
-          uint4 v[4];
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(to + hf * 32, r);
+            tmem_ld_wait();
+            uint4 v[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v[j].x = pack_half2(__uint_as_float(r[8 * j]) * inv, __uint_as_float(r[8 * j + 1]) * inv);
-            v[j].y = pack_half2(__uint_as_float(r[8 * j + 2]) * inv, __uint_as_float(r[8 * j + 3]) * inv);
-            v[j].z = pack_half2(__uint_as_float(r[8 * j + 4]) * inv, __uint_as_float(r[8 * j + 5]) * inv);
-            v[j].w = pack_half2(__uint_as_float(r[8 * j + 6]) * inv, __uint_as_float(r[8 * j + 7]) * inv);
+            for (int j = 0; j < 4; ++j) {
+              v[j].x = pack_half2(__uint_as_float(r[8 * j]) * inv, __uint_as_float(r[8 * j + 1]) * inv);
+              v[j].y = pack_half2(__uint_as_float(r[8 * j + 2]) * inv, __uint_as_float(r[8 * j + 3]) * inv);
+              v[j].z = pack_half2(__uint_as_float(r[8 * j + 4]) * inv, __uint_as_float(r[8 * j + 5]) * inv);
+              v[j].w = pack_half2(__uint_as_float(r[8 * j + 6]) * inv, __uint_as_float(r[8 * j + 7]) * inv);
+            }
+            if (piece) {
+              uint4* po = reinterpret_cast<uint4*>(p.part_o + (static_cast<size_t>(blockIdx.x) * kQ + r_in) * kD);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) __stcg(po + 4 * hf + j, v[j]);
+            } else if (qrow < p.Sq) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + 32 * hf + 8 * j) = v[j];
+            }
           }
-          if (piece) {
-            uint4* po = reinterpret_cast<uint4*>(p.part_o + (static_cast<size_t>(blockIdx.x) * kQ + r_in) * kD);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) __stcg(po + 4 * hf + j, v[j]);
-          } else if (qrow < p.Sq) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(dst + 32 * hf + 8 * j) = v[j];
-          }
-        }
         }
         tc_fence_before();
         mbar_arrive(&o_empty[t]);
